@@ -1,0 +1,438 @@
+// Layer norm over the last dimension, forward and backward.
+//
+//   forward    mu = mean(x),  r = 1 / sqrt(mean((x - mu)^2) + eps),  xhat = (x - mu) r,  y = xhat w + b
+//   backward   g = dy w,  dx = r (g - mean(g) - xhat mean(g xhat)),  dw = sum_rows dy xhat,  db = sum_rows dy
+//
+// Both are bound by memory: the forward reads x and writes y, the backward reads x and dy and writes dx.  A row is read once and stays in
+// registers, so the variance is the centred one at no extra traffic (the difference of two large sums would lose it where |mu| is large).
+// A group of threads holds a row, E elements per thread: a warp where the row fits one, whole warps that meet at a barrier of their own otherwise.
+// In the backward a thread keeps its columns over all rows of its group, so the weight sums stay in registers; groups of a CTA are added in shared
+// memory, CTAs by a second kernel in a fixed order (no atomics: the sums have the same bits in every run).  The next row is on its way while the current
+// one is reduced.  All sums are fp32.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "host.h"
+#include "launch.cuh"
+
+namespace q38 {
+
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+enum ParamType : int { PARAM_NONE = 0, PARAM_F32 = 1, PARAM_BF16 = 2, PARAM_F16 = 3 };
+
+struct LnArgs {
+  const void *x, *w, *b, *dy;
+  void* out;                       // y or dx
+  float *mean, *rstd, *partial;    // [rows], [rows], [CTAs][2][dim]
+  long long rows, ldx, lddy;
+  int dim, wt, bt, groups;         // groups of threads per CTA
+  float eps;
+};
+
+template <typename T, int VEC> struct alignas(VEC * sizeof(T)) LnPack { T v[VEC]; };
+
+// VEC parameters at `at` in fp32; the type is one for the launch, so the branch is uniform
+template <int VEC>
+__device__ __forceinline__ void ln_param(const void* p, int type, int at, float (&out)[VEC], float none) {
+  if (type == PARAM_F32) {
+    const LnPack<float, VEC> v = reinterpret_cast<const LnPack<float, VEC>*>(reinterpret_cast<const float*>(p) + at)[0];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = v.v[i];
+  } else if (type == PARAM_BF16) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[at + i]);
+  } else if (type == PARAM_F16) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = __half2float(reinterpret_cast<const __half*>(p)[at + i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[i] = none;
+  }
+}
+
+// Sums of a and b over a group of G threads.  `scratch` belongs to the group (2 x 32 pairs, used in turn, so that one barrier per sum is enough:
+// a thread writes a half again only after a barrier that all reach after they have read it).
+template <bool WARP>
+__device__ __forceinline__ float2 ln_group_sum(float a, float b, float2* scratch, int& turn, int G, int group) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+  if constexpr (!WARP) {
+    const int t = threadIdx.x - group * G, warps = G >> 5;
+    float2* s = scratch + turn * 32;
+    turn ^= 1;
+    if ((t & 31) == 0) s[t >> 5] = make_float2(a, b);
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(G) : "memory");
+    const float2 v = (t & 31) < warps ? s[t & 31] : make_float2(0.f, 0.f);
+    a = v.x; b = v.y;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+  }
+  return make_float2(a, b);
+}
+
+template <typename InT, typename OutT, int VEC, int E, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) layer_norm_fwd_kernel(LnArgs p) {
+  grid_wait();
+  __shared__ float2 scratch[8][64];
+  const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
+  const long long row = (long long)blockIdx.x * p.groups + group;
+  if (row >= p.rows) return;                                     // whole groups leave; their barrier is their own
+  const InT* x = reinterpret_cast<const InT*>(p.x) + row * p.ldx;
+  OutT* y = reinterpret_cast<OutT*>(p.out) + row * p.dim;
+  int turn = 0;
+  float v[E];
+  float sum = 0.f;
+#pragma unroll
+  for (int c = 0; c < E / VEC; ++c) {
+    const int at = (c * G + t) * VEC;
+    if (at < p.dim) {
+      const LnPack<InT, VEC> in = *reinterpret_cast<const LnPack<InT, VEC>*>(x + at);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { v[c * VEC + i] = to_float(in.v[i]); sum += v[c * VEC + i]; }
+    }
+  }
+  const float mu = ln_group_sum<WARP>(sum, 0.f, scratch[WARP ? 0 : group], turn, G, group).x / p.dim;
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < E / VEC; ++c) {
+    if ((c * G + t) * VEC < p.dim) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) { v[c * VEC + i] -= mu; ss += v[c * VEC + i] * v[c * VEC + i]; }
+    }
+  }
+  const float r = rsqrtf(ln_group_sum<WARP>(ss, 0.f, scratch[WARP ? 0 : group], turn, G, group).x / p.dim + p.eps);
+  if (t == 0 && p.mean != nullptr) { p.mean[row] = mu; p.rstd[row] = r; }
+#pragma unroll
+  for (int c = 0; c < E / VEC; ++c) {
+    const int at = (c * G + t) * VEC;
+    if (at < p.dim) {
+      float w[VEC], b[VEC];
+      ln_param<VEC>(p.w, p.wt, at, w, 1.f);
+      ln_param<VEC>(p.b, p.bt, at, b, 0.f);
+      LnPack<OutT, VEC> o;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o.v[i] = from_float<OutT>(v[c * VEC + i] * r * w[i] + b[i]);
+      *reinterpret_cast<LnPack<OutT, VEC>*>(y + at) = o;
+    }
+  }
+}
+
+// ACC: where the weight sums of a thread's columns live (registers, or shared memory for rows so long that registers would spill; each cell has one owner).
+template <typename InT, typename OutT, int VEC, int E, bool WARP, bool ACC_SMEM>
+__global__ void __launch_bounds__(ACC_SMEM ? 1024 : 512, 1) layer_norm_bwd_kernel(LnArgs p) {
+  grid_wait();
+  extern __shared__ float sums[];                                // [2][dim]
+  __shared__ float2 scratch[16][64];
+  constexpr int N = E / VEC;
+  const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
+  const bool wanted = p.partial != nullptr;
+  float aw[ACC_SMEM ? 1 : E], ab[ACC_SMEM ? 1 : E];
+  if constexpr (ACC_SMEM) {
+    for (int i = threadIdx.x; i < 2 * p.dim; i += blockDim.x) sums[i] = 0.f;
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
+  }
+  const long long stride = (long long)gridDim.x * p.groups;
+  long long row = (long long)blockIdx.x * p.groups + group;
+  LnPack<InT, VEC> nx[N];
+  LnPack<OutT, VEC> nd[N];
+  float nmu = 0.f, nr = 0.f;
+  auto fetch = [&](long long at_row) {
+    if (at_row >= p.rows) return;
+    const InT* x = reinterpret_cast<const InT*>(p.x) + at_row * p.ldx;
+    const OutT* d = reinterpret_cast<const OutT*>(p.dy) + at_row * p.lddy;
+    nmu = p.mean[at_row]; nr = p.rstd[at_row];
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int at = (c * G + t) * VEC;
+      if (at < p.dim) {
+        nx[c] = *reinterpret_cast<const LnPack<InT, VEC>*>(x + at);
+        nd[c] = *reinterpret_cast<const LnPack<OutT, VEC>*>(d + at);
+      }
+    }
+  };
+  if (!ACC_SMEM) fetch(row);
+  int turn = 0;
+  for (; row < p.rows; row += stride) {
+    if (ACC_SMEM) fetch(row);                                    // 64 registers per thread: none for a row ahead
+    float hat[E], g[E];
+    const float mu = nmu, r = nr;
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int at = (c * G + t) * VEC;
+      if (at < p.dim) {
+        float w[VEC];
+        ln_param<VEC>(p.w, p.wt, at, w, 1.f);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const int e = c * VEC + i;
+          const float d = to_float(nd[c].v[i]);
+          hat[e] = (to_float(nx[c].v[i]) - mu) * r;
+          if constexpr (ACC_SMEM) { sums[at + i] += d * hat[e]; sums[p.dim + at + i] += d; }
+          else { aw[e] += d * hat[e]; ab[e] += d; }
+          g[e] = d * w[i];
+          s1 += g[e]; s2 += g[e] * hat[e];
+        }
+      }
+    }
+    if (!ACC_SMEM) fetch(row + stride);
+    const float2 s = ln_group_sum<WARP>(s1, s2, scratch[WARP ? 0 : group], turn, G, group);
+    if (p.out == nullptr) continue;
+    const float m1 = s.x / p.dim, m2 = s.y / p.dim;
+    InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int at = (c * G + t) * VEC;
+      if (at < p.dim) {
+        LnPack<InT, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o.v[i] = from_float<InT>(r * (g[c * VEC + i] - m1 - hat[c * VEC + i] * m2));
+        *reinterpret_cast<LnPack<InT, VEC>*>(dx + at) = o;
+      }
+    }
+  }
+  if (!wanted) return;
+  float* mine = p.partial + (long long)blockIdx.x * 2 * p.dim;
+  if constexpr (!ACC_SMEM) {
+    for (int k = 0; k < p.groups; ++k) {                         // groups add in turn: a fixed order
+      __syncthreads();
+      if (k != group) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int at = ((e / VEC) * G + t) * VEC + e % VEC;
+        if (at < p.dim) {
+          if (p.groups == 1) { mine[at] = aw[e]; mine[p.dim + at] = ab[e]; }
+          else { sums[at] = (k ? sums[at] : 0.f) + aw[e]; sums[p.dim + at] = (k ? sums[p.dim + at] : 0.f) + ab[e]; }
+        }
+      }
+    }
+    if (p.groups == 1) return;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * p.dim; i += blockDim.x) mine[i] = sums[i];
+}
+
+// Rows of any length, a CTA each, read again for every sum (the row comes from L2).  The weight sums are kept in the CTA's part of `partial`.
+template <typename InT, typename OutT>
+__global__ void __launch_bounds__(1024) layer_norm_long_kernel(LnArgs p, bool backward) {
+  grid_wait();
+  __shared__ float scratch[32];
+  float* mine = p.partial == nullptr ? nullptr : p.partial + (long long)blockIdx.x * 2 * p.dim;
+  if (mine != nullptr)
+    for (int i = threadIdx.x; i < 2 * p.dim; i += blockDim.x) mine[i] = 0.f;      // a cell is touched by one thread only
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const InT* x = reinterpret_cast<const InT*>(p.x) + row * p.ldx;
+    float w[1], b[1];
+    if (!backward) {
+      float sum = 0.f, ss = 0.f;
+      for (int i = threadIdx.x; i < p.dim; i += blockDim.x) sum += to_float(x[i]);
+      const float mu = block_sum(sum, scratch) / p.dim;
+      for (int i = threadIdx.x; i < p.dim; i += blockDim.x) { const float d = to_float(x[i]) - mu; ss += d * d; }
+      const float r = rsqrtf(block_sum(ss, scratch) / p.dim + p.eps);
+      if (threadIdx.x == 0 && p.mean != nullptr) { p.mean[row] = mu; p.rstd[row] = r; }
+      OutT* y = reinterpret_cast<OutT*>(p.out) + row * p.dim;
+      for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
+        ln_param<1>(p.w, p.wt, i, w, 1.f);
+        ln_param<1>(p.b, p.bt, i, b, 0.f);
+        y[i] = from_float<OutT>((to_float(x[i]) - mu) * r * w[0] + b[0]);
+      }
+    } else {
+      const OutT* dy = reinterpret_cast<const OutT*>(p.dy) + row * p.lddy;
+      const float mu = p.mean[row], r = p.rstd[row];
+      float s1 = 0.f, s2 = 0.f;
+      for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
+        ln_param<1>(p.w, p.wt, i, w, 1.f);
+        const float d = to_float(dy[i]), hat = (to_float(x[i]) - mu) * r;
+        s1 += d * w[0]; s2 += d * w[0] * hat;
+        if (mine != nullptr) { mine[i] += d * hat; mine[p.dim + i] += d; }
+      }
+      const float m1 = block_sum(s1, scratch) / p.dim, m2 = block_sum(s2, scratch) / p.dim;
+      if (p.out == nullptr) continue;
+      InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
+      for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
+        ln_param<1>(p.w, p.wt, i, w, 1.f);
+        dx[i] = from_float<InT>(r * (to_float(dy[i]) * w[0] - m1 - (to_float(x[i]) - mu) * r * m2));
+      }
+    }
+  }
+}
+
+// dw and db from the CTAs' parts: 32 columns per CTA, sixteen threads per column in strides of sixteen parts, then in order.
+__global__ void __launch_bounds__(512) layer_norm_sums_kernel(const float* __restrict__ partial, int parts, int dim, void* dw, int wt, void* db, int bt) {
+  grid_wait();
+  __shared__ float acc[16][33];
+  const int col = blockIdx.x * 32 + threadIdx.x, which = blockIdx.y;
+  float s = 0.f;
+  if (col < dim)
+    for (int q = threadIdx.y; q < parts; q += 16) s += partial[((long long)q * 2 + which) * dim + col];
+  acc[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y != 0 || col >= dim) return;
+  s = 0.f;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) s += acc[q][threadIdx.x];
+  void* to = which ? db : dw;
+  const int type = which ? bt : wt;
+  if (to == nullptr) return;
+  if (type == PARAM_F32) reinterpret_cast<float*>(to)[col] = s;
+  else if (type == PARAM_BF16) reinterpret_cast<__nv_bfloat16*>(to)[col] = __float2bfloat16_rn(s);
+  else reinterpret_cast<__half*>(to)[col] = __float2half_rn(s);
+}
+
+namespace {
+
+int param_type(const c10::optional<at::Tensor>& t) {
+  if (!t.has_value()) return PARAM_NONE;
+  return t->scalar_type() == at::kFloat ? PARAM_F32 : t->scalar_type() == at::kBFloat16 ? PARAM_BF16 : PARAM_F16;
+}
+const void* param_ptr(const c10::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr int LN_LONGEST = 16384;          // longest row that a CTA of 1024 threads holds in registers
+
+// Threads per row: elements come in vectors, a thread holds E of them
+int group_of(int dim, int E) { return (dim + 32 * E - 1) / (32 * E) * 32; }
+
+// Calls f(InT, OutT) for the supported pairs of input and output type.
+template <typename F>
+void by_type(at::ScalarType in, at::ScalarType out, F&& f) {
+  if (in == at::kFloat && out == at::kFloat) f(float{}, float{});
+  else if (in == at::kFloat && out == at::kBFloat16) f(float{}, __nv_bfloat16{});
+  else if (in == at::kBFloat16 && out == at::kBFloat16) f(__nv_bfloat16{}, __nv_bfloat16{});
+  else if (in == at::kHalf && out == at::kHalf) f(__half{}, __half{});
+  else TORCH_CHECK(false, "layer_norm: output type ", out, " for an input of type ", in, " is not supported");
+}
+
+template <typename InT, typename OutT, int VEC>
+void launch_fwd(LnArgs& p, cudaStream_t stream) {
+  // A warp per row up to 1024 elements: no barrier.  Eight rows per CTA.
+  auto warp_rows = [&](auto kernel) { p.groups = 8; launch(kernel, (unsigned)((p.rows + 7) / 8), 256, 0, stream, p); };
+  if (p.dim <= 256) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, 8, true>);
+  else if (p.dim <= 512) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, 16, true>);
+  else if (p.dim <= 1024) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, 32, true>);
+  else {
+    const bool wide = p.dim > 8192;
+    const int G = group_of(p.dim, wide ? 16 : 8);
+    p.groups = std::max(1, std::min(8, 256 / G));
+    const unsigned grid = (unsigned)((p.rows + p.groups - 1) / p.groups);
+    if (wide) launch(layer_norm_fwd_kernel<InT, OutT, VEC, 16, false>, grid, G * p.groups, 0, stream, p);
+    else launch(layer_norm_fwd_kernel<InT, OutT, VEC, 8, false>, grid, G * p.groups, 0, stream, p);
+  }
+}
+
+struct BwdShape { int G, groups, ctas; };
+BwdShape bwd_shape(long long rows, int dim) {
+  BwdShape s;
+  if (dim > LN_LONGEST) return {1024, 1, (int)std::min<long long>(rows, kNumSMs)};
+  s.G = dim <= 512 ? 32 : group_of(dim, dim <= 4096 ? 8 : 16);
+  s.groups = std::max(1, 512 / s.G);
+  s.ctas = (int)std::min<long long>((rows + s.groups - 1) / s.groups, (s.G * s.groups > 512 ? 1 : 2) * kNumSMs);
+  return s;
+}
+
+template <typename InT, typename OutT, int VEC>
+void launch_bwd(LnArgs& p, const BwdShape& s, cudaStream_t stream) {
+  p.groups = s.groups;
+  const size_t smem = (s.groups > 1 || p.dim > 8192) ? size_t(2) * p.dim * 4 : 0;
+  auto go = [&](auto kernel) {
+    if (smem > 40 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    launch(kernel, (unsigned)s.ctas, s.G * s.groups, smem, stream, p);
+  };
+  if (p.dim <= 256) go(layer_norm_bwd_kernel<InT, OutT, VEC, 8, true, false>);
+  else if (p.dim <= 512) go(layer_norm_bwd_kernel<InT, OutT, VEC, 16, true, false>);
+  else if (p.dim <= 4096) go(layer_norm_bwd_kernel<InT, OutT, VEC, 8, false, false>);
+  else if (p.dim <= 8192) go(layer_norm_bwd_kernel<InT, OutT, VEC, 16, false, false>);
+  else go(layer_norm_bwd_kernel<InT, OutT, VEC, 16, false, true>);
+}
+
+void check_params(const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b) {
+  for (const auto* t : {&w, &b})
+    if (t->has_value())
+      TORCH_CHECK((*t)->device() == x.device() && (*t)->dim() == 1 && (*t)->size(0) == x.size(1) && (*t)->is_contiguous() &&
+                  ((*t)->scalar_type() == at::kFloat || (*t)->scalar_type() == at::kBFloat16 || (*t)->scalar_type() == at::kHalf),
+                  "layer_norm: weight and bias are contiguous fp32, bf16 or fp16 vectors of the last dimension's length on the input's device");
+}
+
+}  // namespace
+
+// x [rows, dim] with contiguous columns -> {y, mean, rstd}; without `save` the last two are empty.
+std::vector<at::Tensor> layer_norm_fwd(const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b, double eps, at::ScalarType out_type, bool save) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) > 0 && (x.stride(1) == 1 || x.size(1) == 1) && x.size(1) <= INT_MAX / 2, "layer_norm: [rows, dim] CUDA input with contiguous columns required");
+  check_params(x, w, b);
+  const c10::cuda::CUDAGuard guard(x.device());
+  LnArgs p{};
+  p.rows = x.size(0); p.dim = (int)x.size(1); p.ldx = x.stride(0); p.eps = (float)eps;
+  auto y = at::empty({p.rows, p.dim}, x.options().dtype(out_type));
+  auto stats = at::empty({save ? 2 : 0, p.rows}, x.options().dtype(at::kFloat));
+  auto mean = save ? stats[0] : stats, rstd = save ? stats[1] : stats;
+  p.x = x.data_ptr(); p.out = y.data_ptr(); p.w = param_ptr(w); p.b = param_ptr(b); p.wt = param_type(w); p.bt = param_type(b);
+  if (save) { p.mean = mean.data_ptr<float>(); p.rstd = rstd.data_ptr<float>(); }
+  by_type(x.scalar_type(), out_type, [&](auto in, auto out) {
+    using InT = decltype(in);
+    using OutT = decltype(out);
+    constexpr int VEC = 16 / sizeof(InT);
+    if (p.rows == 0) return;
+    TORCH_CHECK(p.rows < (1ll << 31), "layer_norm: at most 2^31 - 1 rows");
+    auto stream = at::cuda::getCurrentCUDAStream();
+    const bool vec = p.dim % VEC == 0 && p.ldx % VEC == 0 && on16(p.x) && on16(p.out) && on16(p.w) && on16(p.b);
+    if (p.dim > LN_LONGEST) launch(layer_norm_long_kernel<InT, OutT>, (unsigned)std::min<long long>(p.rows, 2 * kNumSMs), 1024, 0, stream, p, false);
+    else if (vec) launch_fwd<InT, OutT, VEC>(p, stream);
+    else launch_fwd<InT, OutT, 1>(p, stream);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    count_launch();
+  });
+  return {y, mean, rstd};
+}
+
+// {dx, dw, db}: empty where not wanted.
+std::vector<at::Tensor> layer_norm_bwd(const at::Tensor& dy, const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b, const at::Tensor& mean,
+                                       const at::Tensor& rstd, bool want_dx, bool want_dw, bool want_db) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1) && dy.device() == x.device() && dy.sizes() == x.sizes() && (dy.stride(1) == 1 || dy.size(1) == 1) &&
+              mean.numel() == x.size(0) && rstd.numel() == x.size(0), "layer_norm_bwd: bad inputs");
+  check_params(x, w, b);
+  const c10::cuda::CUDAGuard guard(x.device());
+  LnArgs p{};
+  p.rows = x.size(0); p.dim = (int)x.size(1); p.ldx = x.stride(0); p.lddy = dy.stride(0);
+  auto dx = want_dx ? at::empty({p.rows, p.dim}, x.options()) : at::Tensor();
+  auto dw = want_dw ? at::empty_like(*w) : at::Tensor(), db = want_db ? at::empty_like(*b) : at::Tensor();
+  if (p.rows == 0) {
+    if (want_dw) dw.zero_();
+    if (want_db) db.zero_();
+    return {dx, dw, db};
+  }
+  const BwdShape s = bwd_shape(p.rows, p.dim);
+  at::Tensor partial;
+  if (want_dw || want_db) partial = at::empty({s.ctas, 2, p.dim}, x.options().dtype(at::kFloat));
+  p.x = x.data_ptr(); p.dy = dy.data_ptr(); p.w = param_ptr(w); p.wt = param_type(w);
+  p.out = want_dx ? dx.data_ptr() : nullptr;
+  p.mean = mean.data_ptr<float>(); p.rstd = rstd.data_ptr<float>(); p.partial = partial.defined() ? partial.data_ptr<float>() : nullptr;
+  auto stream = at::cuda::getCurrentCUDAStream();
+  by_type(x.scalar_type(), dy.scalar_type(), [&](auto in, auto out) {
+    using InT = decltype(in);
+    using OutT = decltype(out);
+    constexpr int VEC = 16 / sizeof(InT);
+    const bool vec = p.dim % VEC == 0 && p.ldx % VEC == 0 && p.lddy % VEC == 0 && on16(p.x) && on16(p.dy) && on16(p.out) && on16(p.w);
+    if (p.dim > LN_LONGEST) launch(layer_norm_long_kernel<InT, OutT>, (unsigned)s.ctas, 1024, 0, stream, p, true);
+    else if (vec) launch_bwd<InT, OutT, VEC>(p, s, stream);
+    else launch_bwd<InT, OutT, 1>(p, s, stream);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    count_launch();
+  });
+  if (partial.defined()) {
+    launch(layer_norm_sums_kernel, dim3((p.dim + 31) / 32, 2), dim3(32, 16), 0, stream, (const float*)p.partial, s.ctas, p.dim, want_dw ? dw.data_ptr() : nullptr,
+           param_type(w), want_db ? db.data_ptr() : nullptr, param_type(b));
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    count_launch();
+  }
+  return {dx, dw, db};
+}
+
+}  // namespace q38

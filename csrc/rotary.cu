@@ -1,0 +1,199 @@
+// Rotary positions of queries and keys in one launch.
+//
+//   pair i of a head at position t:  a' = m (a cos(t f_i) - b sin(t f_i)),  b' = m (b cos(t f_i) + a sin(t f_i))
+//
+// where the pair is (x[i], x[i + r/2]) or, interleaved, (x[2i], x[2i + 1]); elements from r on pass through.  The gradient is the same with
+// the opposite angle.  Frequencies f come from the caller in 64 bits (however they were scaled) and angles are reduced to turns in 64 bits: at
+// position 10^6 an angle in 32 bits is off by 0.03.
+//
+// Bound by memory: every element is read and written once.  A CTA takes a few tokens, makes their cosines and sines once for all heads (shared memory), and
+// walks the tokens' heads in pieces of 16 bytes: a piece of each half, two neighbouring pieces of an interleaved head, or two that pass through.
+// Tensors are addressed by their strides, so packed projections and head-major tensors are read in place.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "host.h"
+#include "launch.cuh"
+
+namespace q38 {
+
+template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+struct RotarySide {               // queries or keys: strides of batch, token and head
+  const void* in;
+  void* out;
+  long long in_b, in_s, in_h, out_b, out_s, out_h;
+};
+struct RotaryArgs {
+  RotarySide q, k;
+  const double* freq;             // [r / 2]
+  const void* pos;                // [batch or 1, tokens], 32 or 64 bits
+  long long pos_b, pos_s, tokens; // tokens = batch * seq
+  int seq, q_heads, heads, dim, half, units, per_cta, pos64;      // heads of both sides; units per head
+  float magnitude, sign;
+};
+
+constexpr int ROT_THREADS = 256, ROT_BATCH = 4;
+
+template <typename T, int VEC> struct alignas(VEC * sizeof(T)) RotPack { T v[VEC]; };
+
+// VEC == 1: a unit is one pair, or one element that passes through.  VEC > 1: two packs: one of each half, two neighbours of an interleaved head, or two
+// (the last unit perhaps one) that pass through.
+template <typename T, int VEC, bool INTERLEAVED>
+__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotaryArgs p) {
+  grid_wait();
+  extern __shared__ float2 turns[];                      // [per_cta][half]: cos, sin
+  const long long first = (long long)blockIdx.x * p.per_cta;
+  const int count = (int)min((long long)p.per_cta, p.tokens - first);
+  for (int i = threadIdx.x; i < count * p.half; i += ROT_THREADS) {
+    const int local = i / p.half, f = i - local * p.half;
+    const long long token = first + local, b = token / p.seq, s = token - b * p.seq;
+    const long long at = b * p.pos_b + s * p.pos_s;
+    const double t = p.pos64 ? (double)reinterpret_cast<const long long*>(p.pos)[at] : (double)reinterpret_cast<const int*>(p.pos)[at];
+    const double turn = t * (p.freq[f] * 0.15915494309189533576888);            // 1 / (2 pi)
+    float sn, cs;
+    sincospif(2.f * (float)(turn - rint(turn)), &sn, &cs);
+    turns[i] = make_float2(cs * p.magnitude, sn * p.magnitude * p.sign);
+  }
+  __syncthreads();
+
+  constexpr int PACKS = 2;
+  const int rot_units = VEC == 1 ? p.half : p.half / VEC;
+  const int total = count * p.heads * p.units;
+  for (int base = threadIdx.x; base < total; base += ROT_THREADS * ROT_BATCH) {
+    RotPack<T, VEC> v[ROT_BATCH][PACKS];
+    const T* src[ROT_BATCH];
+    T* dst[ROT_BATCH];
+    int second[ROT_BATCH], angle[ROT_BATCH];             // distance of the second pack (0: there is none); first angle, or -1 where elements pass through
+#pragma unroll
+    for (int j = 0; j < ROT_BATCH; ++j) {
+      const int i = base + j * ROT_THREADS;
+      src[j] = nullptr;
+      if (i < total) {
+        const int row = i / p.units, unit = i - row * p.units, local = row / p.heads, head = row - local * p.heads;
+        const long long token = first + local, b = token / p.seq, s = token - b * p.seq;
+        const bool key = head >= p.q_heads;
+        const RotarySide& side = key ? p.k : p.q;
+        const int h = key ? head - p.q_heads : head;
+        int at;
+        if (unit < rot_units) {
+          at = INTERLEAVED ? 2 * VEC * unit : VEC * unit;
+          second[j] = INTERLEAVED ? VEC : p.half;
+          angle[j] = local * p.half + unit * VEC;
+        } else {
+          const int rest = unit - rot_units;
+          at = 2 * p.half + (VEC == 1 ? rest : 2 * VEC * rest);
+          second[j] = VEC > 1 && at + VEC < p.dim ? VEC : 0;
+          angle[j] = -1;
+        }
+        src[j] = reinterpret_cast<const T*>(side.in) + b * side.in_b + s * side.in_s + h * side.in_h + at;
+        dst[j] = reinterpret_cast<T*>(side.out) + b * side.out_b + s * side.out_s + h * side.out_h + at;
+        v[j][0] = *reinterpret_cast<const RotPack<T, VEC>*>(src[j]);
+        if (second[j]) v[j][1] = *reinterpret_cast<const RotPack<T, VEC>*>(src[j] + second[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < ROT_BATCH; ++j) {
+      if (src[j] == nullptr) continue;
+      if (angle[j] >= 0) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float2 cs = turns[angle[j] + e];
+          T& lo = INTERLEAVED && VEC > 1 ? v[j][2 * e / VEC].v[2 * e % VEC] : v[j][0].v[e];
+          T& hi = INTERLEAVED && VEC > 1 ? v[j][(2 * e + 1) / VEC].v[(2 * e + 1) % VEC] : v[j][1].v[e];
+          const float a = to_float(lo), b = to_float(hi);
+          lo = from_float<T>(a * cs.x - b * cs.y);
+          hi = from_float<T>(b * cs.x + a * cs.y);
+        }
+      }
+      *reinterpret_cast<RotPack<T, VEC>*>(dst[j]) = v[j][0];
+      if (second[j]) *reinterpret_cast<RotPack<T, VEC>*>(dst[j] + second[j]) = v[j][1];
+    }
+  }
+}
+
+namespace {
+
+using at::Tensor;
+
+Tensor with_columns(const Tensor& t) { return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous(); }
+
+RotarySide side_of(const Tensor& in, const Tensor& out) {
+  return {in.data_ptr(), out.data_ptr(), in.stride(0), in.stride(1), in.stride(2), out.stride(0), out.stride(1), out.stride(2)};
+}
+bool packs_fit(const Tensor& t, int vec) {
+  return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(0) % vec == 0 && t.stride(1) % vec == 0 && t.stride(2) % vec == 0;
+}
+
+template <typename T>
+void launch_rotary(RotaryArgs& p, bool fit, bool interleaved, cudaStream_t stream) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int rest = p.dim - 2 * p.half;
+  const bool vec = fit && p.dim % VEC == 0 && p.half % VEC == 0;
+  p.units = vec ? p.half / VEC + (rest / VEC + 1) / 2 : p.half + rest;
+  // Tokens per CTA: eight units per thread (two batches of loads), fewer where that leaves an SM without work; their angles fit 32 KB
+  const long long per_token = (long long)p.heads * p.units;
+  long long n = std::max<long long>(1, 8 * ROT_THREADS / per_token);
+  n = std::min(n, std::max<long long>(1, p.tokens / (2 * kNumSMs)));
+  if (p.half) n = std::max<long long>(1, std::min<long long>(n, 4096 / p.half));
+  p.per_cta = (int)n;
+  const long long grid = (p.tokens + n - 1) / n;
+  TORCH_CHECK(grid < (1ll << 31) && per_token * n < (1ll << 30), "rotary: tensor too large");
+  const size_t smem = size_t(p.per_cta) * p.half * sizeof(float2);
+  auto go = [&](auto kernel) {
+    if (smem > 48 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    launch(kernel, (unsigned)grid, ROT_THREADS, smem, stream, p);
+  };
+  if (vec) { if (interleaved) go(rotary_kernel<T, VEC, true>); else go(rotary_kernel<T, VEC, false>); }
+  else { if (interleaved) go(rotary_kernel<T, 1, true>); else go(rotary_kernel<T, 1, false>); }
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  count_launch();
+}
+
+}  // namespace
+
+// q, k [batch, seq, heads, dim] of any strides -> tensors of their layout (either may be absent).  `sign` -1: the gradient.
+std::pair<Tensor, Tensor> rotary_apply(const Tensor& q_in, const Tensor& k_in, const Tensor& pos, const Tensor& freq, double magnitude, bool interleaved, double sign) {
+  const Tensor& any = q_in.defined() ? q_in : k_in;
+  const c10::cuda::CUDAGuard guard(any.device());
+  Tensor q, k, qo, ko;
+  if (q_in.defined()) { q = with_columns(q_in); qo = at::empty_like(q); }
+  if (k_in.defined()) { k = with_columns(k_in); ko = at::empty_like(k); }
+  RotaryArgs p{};
+  const int vec = 16 / (int)any.element_size();
+  bool fit = true;
+  if (q.defined()) { p.q = side_of(q, qo); fit = fit && packs_fit(q, vec) && packs_fit(qo, vec); }
+  if (k.defined()) { p.k = side_of(k, ko); fit = fit && packs_fit(k, vec) && packs_fit(ko, vec); }
+  p.q_heads = q.defined() ? (int)q.size(2) : 0;
+  p.heads = p.q_heads + (k.defined() ? (int)k.size(2) : 0);
+  p.seq = (int)any.size(1); p.tokens = any.size(0) * any.size(1); p.dim = (int)any.size(3); p.half = (int)freq.size(0);
+  p.freq = freq.data_ptr<double>(); p.pos = pos.data_ptr(); p.pos64 = pos.scalar_type() == at::kLong;
+  p.pos_b = pos.dim() == 2 && pos.size(0) > 1 ? pos.stride(0) : 0; p.pos_s = pos.stride(-1);
+  p.magnitude = (float)magnitude; p.sign = (float)sign;
+  if (p.tokens > 0 && p.heads > 0) {
+    auto stream = at::cuda::getCurrentCUDAStream();
+    if (any.scalar_type() == at::kBFloat16) launch_rotary<__nv_bfloat16>(p, fit, interleaved, stream);
+    else if (any.scalar_type() == at::kHalf) launch_rotary<__half>(p, fit, interleaved, stream);
+    else launch_rotary<float>(p, fit, interleaved, stream);
+  }
+  return {qo, ko};
+}
+
+void rotary_check(const Tensor& q, const c10::optional<Tensor>& k, const Tensor& pos, const Tensor& freq) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf || q.scalar_type() == at::kFloat),
+              "rotary: bf16, fp16 or fp32 CUDA tensors [batch, seq, heads, dim] required");
+  TORCH_CHECK(!k.has_value() || (k->device() == q.device() && k->scalar_type() == q.scalar_type() && k->dim() == 4 && k->size(0) == q.size(0) && k->size(1) == q.size(1) && k->size(3) == q.size(3)),
+              "rotary: keys have the type, device, batch, length and head size of the queries");
+  TORCH_CHECK(pos.device() == q.device() && (pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) &&
+              ((pos.dim() == 1 && pos.size(0) == q.size(1)) || (pos.dim() == 2 && pos.size(1) == q.size(1) && (pos.size(0) == q.size(0) || pos.size(0) == 1))),
+              "rotary: whole positions [seq], [1, seq] or [batch, seq] on the queries' device required");
+  TORCH_CHECK(freq.device() == q.device() && freq.scalar_type() == at::kDouble && freq.dim() == 1 && freq.is_contiguous() && 2 * freq.size(0) <= q.size(3),
+              "rotary: contiguous 64-bit frequencies on the queries' device, at most half a head of them, required");
+  TORCH_CHECK(q.size(1) < (1ll << 31) && q.size(3) <= 8192, "rotary: sequence or head too long");
+}
+
+}  // namespace q38

@@ -126,3 +126,6 @@ def muon_batched_step(views, per_call, lr, momentum, weight_decay, ns_steps, sca
 def launch_count():
     """Kernels launched by this library since it was loaded."""
     return int(load().launch_count())
+
+
+from .training import clip_grad_norm, grad_norm, layer_norm, rotary, rotary_frequencies  # noqa: E402,F401  (needs `load`)
