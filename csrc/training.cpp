@@ -7,6 +7,12 @@
 #include "host.h"
 
 namespace q38 {
+// vocab_loss.cu
+std::vector<at::Tensor> vocab_loss_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, int64_t reduction, const at::Tensor& err);
+std::vector<at::Tensor> vocab_loss_bwd(const at::Tensor& g, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& lse2, const at::Tensor& count,
+                                       int64_t reduction, bool want_dh, bool fp32_dh, bool want_dw, bool fp32_dw, const c10::optional<at::Tensor>& grad, int64_t workspace,
+                                       const at::Tensor& err);
+
 namespace {
 
 using at::Tensor;
@@ -84,6 +90,9 @@ std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& po
 TORCH_LIBRARY_FRAGMENT(q38, m) {
   m.def("layer_norm(Tensor x, Tensor? w, Tensor? b, float eps, ScalarType? out_dtype=None) -> Tensor", &q38::layer_norm);
   m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor frequencies, float magnitude, bool interleaved) -> Tensor[]", &q38::rotary);
+  m.def("vocab_loss_fwd(Tensor hidden, Tensor weight, Tensor target, int reduction, Tensor(a!) err) -> Tensor[]", &q38::vocab_loss_fwd);
+  m.def("vocab_loss_bwd(Tensor g, Tensor hidden, Tensor weight, Tensor target, Tensor lse2, Tensor count, int reduction, bool want_dh, bool fp32_dh, bool want_dw, bool fp32_dw, "
+        "Tensor(b!)? grad, int workspace, Tensor(a!) err) -> Tensor[]", &q38::vocab_loss_bwd);
   m.def("grad_norm(Tensor[] grads) -> Tensor", [](at::TensorList g) { return q38::clip_grad_norm(g, {}, 1.0, false); });
   m.def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm) -> Tensor", [](at::TensorList g, double m) { return q38::clip_grad_norm(g, {}, m, true); });
   m.def("clip_grad_norm_out(Tensor[] grads, Tensor(a!)[] out, float max_norm) -> Tensor", [](at::TensorList g, at::TensorList o, double m) { return q38::clip_grad_norm(g, o, m, true); });

@@ -27,6 +27,39 @@ def linear_cross_entropy(weight, hidden, target, reduction="mean"):
     return F.cross_entropy(logits, target, ignore_index=-100, reduction=reduction)
 
 
+def vocabulary_cross_entropy(weight, hidden, target, reduction="mean"):
+    """Softmax cross entropy of ``hidden @ weight.T`` against ``target`` for vocabularies of any size, without keeping logits.
+
+    hidden: ``[..., h]`` bf16 or fp32 (rounded to bf16 for the products); weight: ``[vocabulary, h]`` bf16, or fp32 as a master weight; target: int64 of
+    hidden's leading shape, -100 where a row does not count (any other target outside the vocabulary counts as -100 and raises at
+    `q38.ops.check_errors`).  ``reduction``: ``"mean"`` over the rows that count (0 where none does), ``"sum"``, or ``"none"`` (fp32 losses of
+    target's shape, 0 where a row does not count).
+
+    On a GPU the scores exist as one piece's bf16 gradients at most; scores, sums and losses are fp32, and results have the same bits in every
+    run.  Where `linear_cross_entropy` keeps bf16 scores of all rows for the backward (vocabularies up to 16384), this forms them again: a quarter more
+    products for memory that does not grow with the vocabulary."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"vocabulary_cross_entropy: reduction must be mean, sum or none, got {reduction!r}")
+    if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or not weight.numel():
+        raise ValueError("vocabulary_cross_entropy: hidden [..., h] and weight [vocabulary, h] required")
+    if target.shape != hidden.shape[:-1] or target.dtype != torch.int64:
+        raise ValueError("vocabulary_cross_entropy: int64 targets of hidden's leading shape required")
+    if hidden.dtype not in (torch.bfloat16, torch.float32) or weight.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("vocabulary_cross_entropy: bf16 or fp32 hidden states and weight required")
+    if weight.device != hidden.device or target.device != hidden.device:
+        raise ValueError("vocabulary_cross_entropy: hidden, weight and target on one device required")
+    h2, t1 = hidden.reshape(-1, hidden.shape[-1]), target.reshape(-1)
+    if hidden.is_cuda:
+        from .ops.vocab import vocabulary_loss
+        loss = vocabulary_loss(h2, weight, t1.contiguous(), reduction)
+        return loss.view(target.shape) if reduction == "none" else loss
+    scores = F.linear(h2, weight.to(h2.dtype)).float()
+    losses = F.cross_entropy(scores, t1, ignore_index=-100, reduction="none")
+    if reduction == "none":
+        return losses.view(target.shape)
+    return losses.sum() if reduction == "sum" else losses.sum() / (t1 != -100).sum().clamp_min(1)
+
+
 class LossModel(torch.nn.Module):
     def __init__(self, lm, experts=None, topk=None, ce=None):
         super().__init__()

@@ -129,3 +129,33 @@ def _pair():
 def test_clip_refuses(call):
     with pytest.raises(ValueError):
         call()
+
+
+# ---- vocabulary loss -----------------------------------------------------------------------------------------------------------------
+def test_vocabulary_loss_formula():
+    from q38.losses import vocabulary_cross_entropy
+    h, w = torch.randn(2, 5, 8, requires_grad=True), torch.randn(11, 8, requires_grad=True)
+    target = torch.randint(0, 11, (2, 5))
+    target[0, 1] = -100
+    logp = torch.log_softmax(h.double() @ w.double().t(), -1)
+    each = torch.where(target < 0, 0.0, -logp.gather(-1, target.clamp_min(0)[..., None])[..., 0])
+    for reduction, want in (("none", each), ("sum", each.sum()), ("mean", each.sum() / 9)):
+        got = vocabulary_cross_entropy(w, h, target, reduction)
+        assert got.shape == want.shape and (got - want).abs().max() < 1e-5
+    dh, dw = torch.autograd.grad(vocabulary_cross_entropy(w, h, target), [h, w])
+    eh, ew = torch.autograd.grad(each.sum() / 9, [h, w])
+    assert (dh - eh).abs().max() < 1e-6 and (dw - ew).abs().max() < 1e-6
+    assert vocabulary_cross_entropy(w, h, torch.full((2, 5), -100)) == 0
+
+
+def _vocab(h=(3, 8), w=(11, 8), t=(3,), ht=torch.float32, wt=torch.float32, tt=torch.int64, reduction="mean"):
+    from q38.losses import vocabulary_cross_entropy
+    return vocabulary_cross_entropy(torch.zeros(w, dtype=wt), torch.zeros(h, dtype=ht), torch.zeros(t, dtype=tt), reduction)
+
+
+@pytest.mark.parametrize("wrong", [dict(h=(3, 7)), dict(h=()), dict(w=(11,)), dict(w=(0, 8)), dict(h=(3, 0), w=(11, 0)), dict(t=(4,)), dict(t=(3, 1)), dict(tt=torch.int32), dict(ht=torch.float16),
+                                   dict(wt=torch.float64), dict(reduction="max")])
+def test_vocabulary_loss_refuses(wrong):
+    _vocab()
+    with pytest.raises(ValueError):
+        _vocab(**wrong)
