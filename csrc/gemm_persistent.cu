@@ -33,6 +33,9 @@ struct PGemmArgs {
   const __nv_bfloat16* Cin;
   long long ldcin, cin_batch_stride;
   float beta;
+  // optional factor from device memory: alpha_num[0], divided by alpha_den[0] where that is given, instead of alpha
+  const float *alpha_num, *alpha_den;
+  bool slabs;                       // every K split has an output matrix of its own (the batch coordinate of C), added up by the caller in order
 };
 
 // TMA_OUT: every epilogue warp stages 32 rows x 32 columns in shared memory (64-byte swizzle for bf16, 128-byte for fp32, both
@@ -144,10 +147,11 @@ __global__ void __launch_bounds__(P_THREADS) gemm_persistent_kernel(const __grid
     const int quarter = warp & 3;
     uint32_t tile = 0, chunk = 0;
     bool ok = true;
+    const float alpha0 = p.alpha_num == nullptr ? p.alpha : p.alpha_den == nullptr ? *p.alpha_num : __fdiv_rn(*p.alpha_num, *p.alpha_den);
     for (int w = blockIdx.x; w < p.work_items && ok; w += gridDim.x, ++tile) {
       int bz, m0, n0, kb_begin, num_kb;
       decode(w, bz, m0, n0, kb_begin, num_kb);
-      const int acc = tile & 1;
+      const int acc = tile & 1, cz = p.slabs ? kb_begin / p.kb_per_split : bz;
       if (!ptx::mbar_wait_warp(&acc_full[acc], (tile >> 1) & 1, 1u << 22)) { report_error(p.err, ERR_EPILOGUE_WAIT); ok = false; break; }
       ptx::tc_fence_after();
       const int row = m0 + quarter * 32 + lane;
@@ -158,7 +162,7 @@ __global__ void __launch_bounds__(P_THREADS) gemm_persistent_kernel(const __grid
         uint32_t r[32];
         ptx::tmem_ld_32x32b_x32(t_addr + c0, r);
         ptx::tmem_ld_wait();
-        float alpha = p.alpha;
+        float alpha = alpha0;
         if constexpr (sizeof(OutT) == 2) {
           if (p.Cin != nullptr) {                              // fold alpha * acc + beta * Cin into the registers
             if (row < p.M) {
@@ -214,8 +218,8 @@ __global__ void __launch_bounds__(P_THREADS) gemm_persistent_kernel(const __grid
           __syncwarp();
           if (lane == 0) {
             if (n0 + c0 < p.N && m0 + quarter * 32 < p.M) {
-              if constexpr (ACCUM) ptx::tma_reduce_add_3d(&tmC, buf, n0 + c0, m0 + quarter * 32, bz);
-              else ptx::tma_store_3d(&tmC, buf, n0 + c0, m0 + quarter * 32, bz);
+              if constexpr (ACCUM) ptx::tma_reduce_add_3d(&tmC, buf, n0 + c0, m0 + quarter * 32, cz);
+              else ptx::tma_store_3d(&tmC, buf, n0 + c0, m0 + quarter * 32, cz);
             }
             ptx::bulk_commit();                                  // possibly empty: keeps the buffer accounting uniform
           }
@@ -343,9 +347,8 @@ static void launch_p(const CUtensorMap& ta, const CUtensorMap& tb, const CUtenso
 bool gemm_pair_enabled();                                                                                                         // gemm_pair.cu
 bool gemm_bf16_pair(const Mat& a, const Mat& b, const Mat& c, double alpha, bool accumulate, int* err);   // gemm_pair.cu
 
-// Same contract as gemm_bf16 (bf16 operands only).
-void gemm_bf16_persistent(const at::Tensor& a_, const at::Tensor& b_, const at::Tensor& c_, bool a_mn_major, bool b_mn_major, double alpha,
-                          bool accumulate, const at::Tensor& err, int64_t splits, const c10::optional<at::Tensor>& addend, double beta) {
+static void gemm_p(const at::Tensor& a_, const at::Tensor& b_, const at::Tensor& c_, bool a_mn_major, bool b_mn_major, double alpha, bool accumulate, const at::Tensor& err,
+                   int64_t splits, const c10::optional<at::Tensor>& addend, double beta, const float* alpha_num, const float* alpha_den, int slabs) {
   const Mat a(a_), b(b_), c(c_);
   const bool tf32 = a.type == at::kFloat;
   TORCH_CHECK((tf32 || a.type == at::kBFloat16) && b.type == a.type, "gemm_bf16_persistent: bf16 (or fp32 for tf32 math) [batch, rows, cols] operands required");
@@ -356,15 +359,16 @@ void gemm_bf16_persistent(const at::Tensor& a_, const at::Tensor& b_, const at::
   const int batch = a.batch;
   const int M = a_mn_major ? a.cols : a.rows, K = a_mn_major ? a.rows : a.cols;
   const int N = b_mn_major ? b.cols : b.rows, Kb = b_mn_major ? b.rows : b.cols;
-  TORCH_CHECK(K == Kb && b.batch == batch && c.batch == batch && c.rows == M && c.cols == N, "gemm_bf16_persistent: shape mismatch");
+  TORCH_CHECK(K == Kb && b.batch == batch && (slabs ? batch == 1 && c.batch == slabs : c.batch == batch) && c.rows == M && c.cols == N, "gemm_bf16_persistent: shape mismatch");
   const bool out_fp32 = c.type == at::kFloat;
   TORCH_CHECK(out_fp32 || c.type == at::kBFloat16, "gemm_bf16_persistent: output must be bf16 or fp32");
   const int c_eb = out_fp32 ? 4 : 2, c_vec = 16 / c_eb;
-  const bool tma_out = c.row_stride % c_vec == 0 && (reinterpret_cast<uintptr_t>(c.ptr) & 15) == 0 && (batch == 1 || c.batch_stride % c_vec == 0);
+  const bool tma_out = c.row_stride % c_vec == 0 && (reinterpret_cast<uintptr_t>(c.ptr) & 15) == 0 && (c.batch == 1 || c.batch_stride % c_vec == 0);
+  TORCH_CHECK(!slabs || tma_out, "gemm_bf16_persistent: separate splits require TMA-storable outputs");
   // bf16 outputs accumulate through the TMA unit only (cp.reduce.async.bulk.tensor adds in the tensor's element type)
   TORCH_CHECK(!accumulate || out_fp32 || (tma_out && !tf32 && !addend.has_value()), "accumulating into a bf16 output requires a TMA-storable output and no addend");
   // K-major x K-major products with a TMA-storable output may run on SM pairs (cta_group::2, gemm_pair.cu) when switched on
-  if (gemm_pair_enabled() && !tf32 && !a_mn_major && !b_mn_major && tma_out && !addend.has_value() && (!accumulate || !out_fp32) &&
+  if (gemm_pair_enabled() && alpha_num == nullptr && !tf32 && !a_mn_major && !b_mn_major && tma_out && !addend.has_value() && (!accumulate || !out_fp32) &&
       gemm_bf16_pair(a, b, c, alpha, accumulate, err.data_ptr<int>()))
     return;
   int bn = pick_bn(N, tma_out ? 32 : 16);
@@ -380,7 +384,9 @@ void gemm_bf16_persistent(const at::Tensor& a_, const at::Tensor& b_, const at::
   // keep 64 KB of A per SM in flight, less than the latency of memory asks for (18 projections of a nine-layer prefill, 16384 x 56 x 1792 tf32: 510 -> 428 us).
   p.stages = std::min(P_MAX_STAGES, (227 * 1024 - 2048 - 4 * 2 * 4096) / (P_BM * 128 + bn * 128));
   int nsplit = 1;
-  if (accumulate && out_fp32) {
+  if (slabs) {
+    nsplit = slabs;
+  } else if (accumulate && out_fp32) {
     if (splits > 0) nsplit = (int)splits;
     else if (splits == 0) {
       const int tiles = p.tiles_m * p.tiles_n * batch;
@@ -389,9 +395,12 @@ void gemm_bf16_persistent(const at::Tensor& a_, const at::Tensor& b_, const at::
   }
   p.kb_per_split = (p.total_kb + nsplit - 1) / nsplit;
   p.splits = (p.total_kb + p.kb_per_split - 1) / p.kb_per_split;
+  TORCH_CHECK(p.splits <= std::max(nsplit, 1), "gemm_bf16_persistent: splits");
   p.work_items = p.tiles_m * p.tiles_n * batch * p.splits;
+  p.slabs = slabs > 0;
   p.C = c.ptr; p.ldc = c.row_stride; p.c_batch_stride = c.batch_stride; p.alpha = (float)alpha; p.err = err.data_ptr<int>();
   p.Cin = nullptr; p.ldcin = 0; p.cin_batch_stride = 0; p.beta = 0.f;
+  p.alpha_num = alpha_num; p.alpha_den = alpha_den;
   if (addend.has_value()) {
     TORCH_CHECK(!out_fp32 && addend->scalar_type() == at::kBFloat16 && addend->dim() == 3 && addend->size(0) == batch && addend->size(1) == M &&
                 addend->size(2) == N && addend->stride(2) == 1, "gemm_bf16_persistent: the addend must be a bf16 tensor of the output's shape (bf16 output only)");
@@ -403,7 +412,7 @@ void gemm_bf16_persistent(const at::Tensor& a_, const at::Tensor& b_, const at::
   Q38_TRACE("[gemm_p] map A encoded\n");
   tb = make_tmap_box(b.ptr, eb, b.cols, b.rows, batch, b.row_stride, b.batch_stride, b_mn_major ? 64 : bn, 128);
   Q38_TRACE("[gemm_p] operand maps encoded\n");
-  CUtensorMap tc = tma_out ? make_tmap_box(c.ptr, c_eb, N, M, batch, c.row_stride, c.batch_stride, 32, 32 * c_eb) : ta;
+  CUtensorMap tc = tma_out ? make_tmap_box(c.ptr, c_eb, N, M, c.batch, c.row_stride, c.batch_stride, 32, 32 * c_eb) : ta;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   if (tf32) {
     launch_p<false, false, true>(ta, tb, tc, tma_out, p, out_fp32, accumulate, stream);
@@ -414,6 +423,25 @@ void gemm_bf16_persistent(const at::Tensor& a_, const at::Tensor& b_, const at::
     if (b_mn_major) launch_p<false, true>(ta, tb, tc, tma_out, p, out_fp32, accumulate, stream);
     else launch_p<false, false>(ta, tb, tc, tma_out, p, out_fp32, accumulate, stream);
   }
+}
+
+// Same contract as gemm_bf16 (bf16 operands only).
+void gemm_bf16_persistent(const at::Tensor& a, const at::Tensor& b, const at::Tensor& c, bool a_mn_major, bool b_mn_major, double alpha, bool accumulate, const at::Tensor& err,
+                          int64_t splits, const c10::optional<at::Tensor>& addend, double beta) {
+  gemm_p(a, b, c, a_mn_major, b_mn_major, alpha, accumulate, err, splits, addend, beta, nullptr, nullptr, 0);
+}
+
+// The same with the factor num[0] / den[0] (den may be null) from device memory, read in the epilogue.  slabs > 0: the reduction is cut into that many parts (fewer
+// where it has fewer blocks of 64), whose products go to c[0], c[1], ...: a long reduction with few output tiles fills the SMs, and the sum over parts keeps one order.
+void gemm_bf16_scaled(const at::Tensor& a, const at::Tensor& b, const at::Tensor& c, bool a_mn_major, bool b_mn_major, const float* num, const float* den, bool accumulate,
+                      int64_t slabs, const at::Tensor& err) {
+  gemm_p(a, b, c, a_mn_major, b_mn_major, 1.0, accumulate, err, -1, c10::nullopt, 0.0, num, den, (int)slabs);
+}
+
+// Output tiles of a product with N columns whose B operand is MN-major.
+int64_t gemm_tiles(int64_t M, int64_t N) {
+  const int bn = std::min(256, (pick_bn((int)N, 32) + 63) / 64 * 64);
+  return (M + P_BM - 1) / P_BM * ((N + bn - 1) / bn);
 }
 
 }  // namespace q38

@@ -6,7 +6,8 @@
 // pair (k, s) with sum = s 2^k and the target's logit; a small kernel joins the pairs.  Nothing of size rows x vocabulary is written.
 // Backward: for one piece of the vocabulary after the other the same tiles are formed again, turned into dz (bf16, a workspace of one piece) and
 // multiplied by W and h on the framework's GEMM.  The logits stay fp32 in tensor memory: storing them in bf16 (half a step of 2^-9 of a logit of ten) would put an
-// error of 2 % into a probability.  dz is rounded to bf16 because the tensor cores take it so; its target entry is -1 + p, whose rounding is small.
+// error of 2 % into a probability.  dz is rounded to bf16 because the tensor cores take it so; its target entry is -1 + p, whose rounding is small, and a factor that all
+// rows share is applied to the products in fp32.
 //
 // The kernel follows csrc/gemm_persistent.cu: one CTA per SM, warp 0 loads by TMA, one lane of warp 1 issues the MMAs into one of two accumulators, and eight
 // warps (two warpgroups on alternate 32-column chunks) read the other.  Tiles are walked with the rows fastest, in groups of rows whose hidden states
@@ -22,6 +23,10 @@
 
 namespace q38 {
 
+void gemm_bf16_scaled(const at::Tensor& a, const at::Tensor& b, const at::Tensor& c, bool a_mn_major, bool b_mn_major, const float* num, const float* den, bool accumulate,
+                      int64_t slabs, const at::Tensor& err);     // gemm_persistent.cu
+int64_t gemm_tiles(int64_t M, int64_t N);                        // gemm_persistent.cu
+
 constexpr int V_BM = 128, V_BK = 64, V_MAX_STAGES = 8, V_THREADS = 320, V_ACC_COLS = 256;
 constexpr float V_LOG2E = 1.44269504088896340736f;
 constexpr long long V_IGNORE = -100;
@@ -32,8 +37,7 @@ struct VocabArgs {
   const long long* target;
   float2* partial;                             // [2 tiles_n][rows]: (k, s) of a half tile
   float* target_logit;                         // [rows]
-  const float *lse2, *upstream, *count;        // backward: log2 of the row's sum; gradient of each row (or of all); divisor (or null)
-  int upstream_step;
+  const float *lse2, *upstream;                // backward: log2 of the row's sum; gradient of each row (null: one factor for all, which the products' epilogues apply)
   int* err;
 };
 
@@ -133,8 +137,7 @@ __global__ void __launch_bounds__(V_THREADS) vocab_tiles_kernel(const __grid_con
       float lse2 = 0.f, scale = 0.f;
       if (GRAD && inside) {
         lse2 = p.lse2[row];
-        scale = p.upstream[(long long)row * p.upstream_step];
-        if (p.count != nullptr) scale = __fdividef(scale, *p.count);
+        scale = p.upstream == nullptr ? 1.f : p.upstream[row];
       }
       if (!ptx::mbar_wait_warp(&acc_full[acc], (tile >> 1) & 1, 1u << 22)) { report_error(p.err, ERR_EPILOGUE_WAIT); ok = false; break; }
       ptx::tc_fence_after();
@@ -231,37 +234,41 @@ __global__ void __launch_bounds__(V_THREADS) vocab_tiles_kernel(const __grid_con
   if (warp == 1) ptx::tmem_dealloc(tmem_base, 512);
 }
 
-// lse2[row] = log2 of the row's sum and loss[row], from the tiles' pairs: 32 rows per CTA, eight threads per row in strides of eight pairs, joined in order.
+// lse2[row] = log2 of the row's sum and loss[row], from the tiles' pairs: 32 rows per CTA, 32 threads per row in strides of 32 pairs, joined in order.
 // A target outside the vocabulary that is not the ignored one is an error: it is reported, and the row counts as ignored.
-__global__ void __launch_bounds__(256) vocab_join_kernel(const float2* __restrict__ partial, int parts, int rows, int vocab, const long long* __restrict__ target,
-                                                         const float* __restrict__ target_logit, float* __restrict__ lse2, float* __restrict__ loss, int* err) {
+__global__ void __launch_bounds__(1024) vocab_join_kernel(const float2* __restrict__ partial, int parts, int rows, int vocab, const long long* __restrict__ target,
+                                                          const float* __restrict__ target_logit, float* __restrict__ lse2, float* __restrict__ loss, int* err) {
   grid_wait();
-  __shared__ float2 part[8][33];
+  __shared__ float2 part[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5, row = blockIdx.x * 32 + x;
   auto join = [](float2 a, float2 b) {
     const float k = fmaxf(a.x, b.x), ref = k == -INFINITY ? 0.f : k;
     return make_float2(k, a.y * exp2_approx(a.x - ref) + b.y * exp2_approx(b.x - ref));
   };
-  float2 v = make_float2(-INFINITY, 0.f);
+  const float2 none = make_float2(-INFINITY, 0.f);
+  float2 v = none;
   if (row < rows) {
-    int i = y;
-    for (; i + 24 < parts; i += 32) {
-      const float2 a = partial[(long long)i * rows + row], b = partial[(long long)(i + 8) * rows + row], c = partial[(long long)(i + 16) * rows + row], d = partial[(long long)(i + 24) * rows + row];
-      v = join(v, join(join(a, b), join(c, d)));
+    for (int i = y; i < parts; i += 128) {                       // four reads in flight
+      float2 r[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) r[q] = i + 32 * q < parts ? partial[(long long)(i + 32 * q) * rows + row] : none;
+      v = join(v, join(join(r[0], r[1]), join(r[2], r[3])));
     }
-    for (; i < parts; i += 8) v = join(v, partial[(long long)i * rows + row]);
   }
   part[y][x] = v;
   __syncthreads();
-  if (y != 0 || row >= rows) return;
+  // a warp per row from here: lane q has the row's part q
+  v = part[x][y];
 #pragma unroll
-  for (int q = 1; q < 8; ++q) v = join(v, part[q][x]);
+  for (int o = 16; o > 0; o >>= 1) v = join(v, make_float2(__shfl_down_sync(0xffffffffu, v.x, o), __shfl_down_sync(0xffffffffu, v.y, o)));
+  const int mine = blockIdx.x * 32 + y;
+  if (x != 0 || mine >= rows) return;
   const double l2 = (double)v.x + log2((double)v.y);
-  const long long tgt = target[row];
+  const long long tgt = target[mine];
   const bool inside = tgt >= 0 && tgt < vocab;
   if (!inside && tgt != V_IGNORE) report_error(err, ERR_BOUNDS);
-  lse2[row] = (float)l2;
-  loss[row] = inside ? (float)(l2 * 0.69314718055994530942 - (double)target_logit[row]) : 0.f;
+  lse2[mine] = (float)l2;
+  loss[mine] = inside ? (float)(l2 * 0.69314718055994530942 - (double)target_logit[mine]) : 0.f;
 }
 
 // Sum of all losses and number of rows that count, by one CTA in a fixed order: out[0] the sum or the mean over those rows, out[1] that number (at least 1).
@@ -286,16 +293,54 @@ __global__ void __launch_bounds__(1024) vocab_sum_kernel(const float* __restrict
   out[1] = (float)n;
 }
 
-// out = sum of `slices` fp32 matrices [rows, cols] (rows of ldp elements), in order, as bf16 or fp32
-__global__ void __launch_bounds__(256) vocab_slices_kernel(const float* __restrict__ part, int slices, long long slice, long long rows, int cols, int ldp, void* out, bool bf16) {
+// out [rows, cols] = sum of `slabs` fp32 matrices (rows of ldp elements, a multiple of 4), in order, as bf16 or fp32: a warp per row, four columns per lane
+template <bool BF16>
+__global__ void __launch_bounds__(256) vocab_slabs_kernel(const float* __restrict__ part, int slabs, long long slab, int rows, int cols, int ldp, void* out) {
   grid_wait();
-  const long long n = rows * cols;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const long long r = i / cols, at = r * ldp + (i - r * cols);
-    float s = part[at];
-    for (int k = 1; k < slices; ++k) s += part[k * slice + at];
-    if (bf16) reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(s);
-    else reinterpret_cast<float*>(out)[i] = s;
+  const int lane = threadIdx.x & 31;
+  const bool packs = cols % 4 == 0;
+  for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8) {
+    const float* in = part + r * ldp;
+#pragma unroll 2
+    for (int c = lane * 4; c < cols; c += 128) {                 // the last pack may end in a row's padding, which is read and not used
+      float4 s = *reinterpret_cast<const float4*>(in + c);
+      for (int k = 1; k < slabs; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(in + k * slab + c);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      }
+      const long long at = r * cols + c;
+      if (packs) {
+        if (BF16) *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(out) + at) = make_uint2(bf16_pair(make_float2(s.x, s.y)), bf16_pair(make_float2(s.z, s.w)));
+        else *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = s;
+      } else {
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < cols) {
+            if (BF16) reinterpret_cast<__nv_bfloat16*>(out)[at + e] = __float2bfloat16_rn(v[e]);
+            else reinterpret_cast<float*>(out)[at + e] = v[e];
+          }
+      }
+    }
+  }
+}
+
+// Rows of bf16 or fp32 into rows of another distance, a warp per row (hidden sizes that TMA does not take, into padded rows and back).
+// torch's copy takes 46 us for 30011 x 711 where this takes a third of it.
+template <typename T>
+__global__ void __launch_bounds__(256) vocab_rows_kernel(const T* __restrict__ in, long long ldi, long long step, T* __restrict__ out, long long ldo, int rows, int cols) {
+  grid_wait();
+  const int lane = threadIdx.x & 31;
+  for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8) {
+    const T* src = in + r * ldi;
+    T* dst = out + r * ldo;
+    for (int base = lane; base < cols; base += 256) {
+      T v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) if (base + 32 * e < cols) v[e] = src[(base + 32 * e) * step];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) if (base + 32 * e < cols) dst[base + 32 * e] = v[e];
+    }
   }
 }
 
@@ -303,20 +348,50 @@ namespace {
 
 using at::Tensor;
 
-// A 2-D bf16 tensor whose rows TMA accepts (contiguous, a multiple of 16 bytes apart, on 16 bytes); others are copied into padded rows
-Tensor tma_rows(const Tensor& t) {
+void copy_rows(const Tensor& in, const Tensor& out, cudaStream_t stream) {
+  const unsigned grid = (unsigned)std::min<int64_t>((in.size(0) + 7) / 8, kNumSMs * 16);
+  if (in.element_size() == 2)
+    launch(vocab_rows_kernel<uint16_t>, grid, 256, 0, stream, (const uint16_t*)in.data_ptr(), in.stride(0), in.stride(1), (uint16_t*)out.data_ptr(), out.stride(0), (int)in.size(0), (int)in.size(1));
+  else
+    launch(vocab_rows_kernel<uint32_t>, grid, 256, 0, stream, (const uint32_t*)in.data_ptr(), in.stride(0), in.stride(1), (uint32_t*)out.data_ptr(), out.stride(0), (int)in.size(0), (int)in.size(1));
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  count_launch();
+}
+
+int64_t padded(int64_t n) { return (n + 63) / 64 * 64; }
+
+// A 2-D bf16 tensor whose rows TMA accepts (contiguous, a multiple of 16 bytes apart, on 16 bytes); others are copied into rows of whole 128-byte lines
+// (rows 16 bytes off a line cost two lines per box: 2049 x 30011 x 711, the tiles' kernel 109 -> 71 us)
+Tensor tma_rows(const Tensor& t, cudaStream_t stream) {
   const int64_t n = t.size(1);
-  if (t.stride(1) == 1 && t.stride(0) >= n && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) return t;
-  auto view = at::empty({t.size(0), (n + 7) / 8 * 8}, t.options()).narrow(1, 0, n);
-  view.copy_(t);
+  if ((t.stride(1) == 1 || n == 1) && (t.stride(0) >= n || t.size(0) == 1) && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) return t;
+  auto view = at::empty({t.size(0), padded(n)}, t.options()).narrow(1, 0, n);
+  copy_rows(t, view, stream);
   return view;
 }
 
-// Tiles of 256 columns, narrower ones where there would not be one for every SM
+// Parts of the reduction of dh = dz W side by side: rounds of tiles times K blocks (0.35 us each, six more for a tile's start), plus the sums' way through memory
+int64_t pick_slabs(int64_t rows, int64_t K, int64_t cols) {
+  const int64_t tiles = gemm_tiles(rows, K), blocks = (cols + 63) / 64;
+  int64_t best = 1;
+  double least = 1e30;
+  for (int64_t s = 1; s <= std::max<int64_t>(8, kNumSMs / tiles) && blocks / s >= 4; ++s) {
+    const int64_t per = (blocks + s - 1) / s;
+    const double cost = double((tiles * s + kNumSMs - 1) / kNumSMs) * (per + 6) * 0.35e-6 + (s > 1 ? double(s) : 0.0) * rows * K * 8 / 6.5e12;
+    if (cost < least * 0.98) { best = (blocks + per - 1) / per; least = cost; }
+  }
+  return best;
+}
+
+// Columns per tile: the fewest rounds of tiles times their width, where a tile's start is worth 32 columns
 int tile_width(int64_t rows, int64_t cols) {
-  int bn = 256;
-  while (bn > 64 && (rows + V_BM - 1) / V_BM * ((cols + bn - 1) / bn) < kNumSMs) bn /= 2;
-  return bn;
+  int best = 256;
+  int64_t least = INT64_MAX;
+  for (int bn = 256; bn >= 64; bn -= 32) {
+    const int64_t items = (rows + V_BM - 1) / V_BM * ((cols + bn - 1) / bn), cost = (items + kNumSMs - 1) / kNumSMs * (bn + 32);
+    if (cost < least) { best = bn; least = cost; }
+  }
+  return best;
 }
 
 template <bool GRAD>
@@ -363,7 +438,7 @@ std::vector<Tensor> vocab_loss_fwd(const Tensor& hidden, const Tensor& weight, c
   auto out = at::empty({reduction ? 2 : 0}, f32);
   auto stream = at::cuda::getCurrentCUDAStream();
   if (rows) {
-    const Tensor h = tma_rows(hidden), w = tma_rows(weight);
+    const Tensor h = tma_rows(hidden, stream), w = tma_rows(weight, stream);
     VocabArgs p{};
     const int bn = tile_width(rows, vocab);
     auto partial = at::empty({2 * ((vocab + bn - 1) / bn), rows, 2}, f32);
@@ -373,7 +448,7 @@ std::vector<Tensor> vocab_loss_fwd(const Tensor& hidden, const Tensor& weight, c
     p.target_logit = logit.data_ptr<float>();
     p.err = err.data_ptr<int>();
     launch_tiles<false>(h, w, 0, vocab, p, nullptr, stream);
-    launch(vocab_join_kernel, (unsigned)((rows + 31) / 32), 256, 0, stream, (const float2*)p.partial, 2 * p.tiles_n, (int)rows, (int)vocab, p.target, (const float*)p.target_logit,
+    launch(vocab_join_kernel, (unsigned)((rows + 31) / 32), 1024, 0, stream, (const float2*)p.partial, 2 * p.tiles_n, (int)rows, (int)vocab, p.target, (const float*)p.target_logit,
            lse2.data_ptr<float>(), loss.data_ptr<float>(), p.err);
     count_launch();
   }
@@ -393,7 +468,7 @@ std::vector<Tensor> vocab_loss_bwd(const Tensor& g, const Tensor& hidden, const 
   TORCH_CHECK(g.device() == hidden.device() && g.scalar_type() == at::kFloat && g.is_contiguous() && g.numel() == (reduction ? 1 : hidden.size(0)) && lse2.numel() == hidden.size(0),
               "vocab_loss_bwd: bad gradient");
   const c10::cuda::CUDAGuard guard(hidden.device());
-  const int64_t rows = hidden.size(0), K = hidden.size(1), vocab = weight.size(0), Kp = (K + 7) / 8 * 8;
+  const int64_t rows = hidden.size(0), K = hidden.size(1), vocab = weight.size(0), Kp = K % 8 ? padded(K) : K;
   const auto f32 = hidden.options().dtype(at::kFloat);
   auto stream = at::cuda::getCurrentCUDAStream();
   Tensor dh, dw;
@@ -402,57 +477,56 @@ std::vector<Tensor> vocab_loss_bwd(const Tensor& g, const Tensor& hidden, const 
     if (want_dw && !grad.has_value()) dw = at::zeros({vocab, K}, fp32_dw ? f32 : weight.options());
     return {dh, dw};
   }
-  const Tensor h = tma_rows(hidden), w = tma_rows(weight);
+  const Tensor h = tma_rows(hidden, stream), w = tma_rows(weight, stream);
   // Pieces: as few as the workspace allows, of equal width (whole tiles)
   const int64_t widest = std::max<int64_t>(256, workspace / (2 * rows) / 256 * 256), pieces = (vocab + widest - 1) / widest;
   const int64_t width = std::min((vocab + 7) / 8 * 8, ((vocab + pieces - 1) / pieces + 255) / 256 * 256);
   auto dz_all = at::empty({rows, width}, hidden.options());
-  // dh: where its tiles are fewer than the SMs, slices of the piece side by side, added in order at the end
-  const int64_t tiles = ((rows + 127) / 128) * ((Kp + 255) / 256);
-  const int64_t slice_cols = std::max<int64_t>(256, (std::max<int64_t>(1, width * tiles / kNumSMs) + 63) / 64 * 64);
-  const int64_t slices = std::max<int64_t>(1, std::min<int64_t>((width + slice_cols - 1) / slice_cols, kNumSMs));
-  const bool direct = want_dh && slices == 1 && pieces == 1;
+  // dh: where its tiles leave SMs without work, parts of the reduction side by side, added in order at the end
+  const int64_t slabs = pick_slabs(rows, K, std::min(width, vocab));
+  const bool direct = want_dh && slabs == 1 && pieces == 1;
   Tensor part;
-  if (want_dh && !direct) part = at::empty({slices, rows, Kp}, f32);
+  if (want_dh && !direct) part = at::empty({slabs, rows, Kp}, f32);
   if (direct) dh = at::empty({rows, Kp}, fp32_dh ? f32 : hidden.options());
   if (want_dw && !grad.has_value()) dw = at::empty({vocab, Kp}, fp32_dw ? f32 : weight.options());
   VocabArgs p{};
   p.target = reinterpret_cast<const long long*>(target.data_ptr<int64_t>());
-  p.lse2 = lse2.data_ptr<float>(); p.upstream = g.data_ptr<float>(); p.upstream_step = reduction ? 0 : 1;
-  p.count = reduction == 2 ? count.data_ptr<float>() : nullptr;
+  p.lse2 = lse2.data_ptr<float>();
+  p.upstream = reduction ? nullptr : g.data_ptr<float>();
   p.err = err.data_ptr<int>();
+  // One factor for all rows stays out of dz: its rounding to bf16 would be the same for every row and not average out (8192 rows, 1/8028: 3.5e-3 instead of 2.2e-3 off)
+  const float* num = reduction ? g.data_ptr<float>() : nullptr;
+  const float* den = reduction == 2 ? count.data_ptr<float>() : nullptr;
   for (int64_t at = 0; at < vocab; at += width) {
     const int64_t cols = std::min(width, vocab - at);
     const bool first = at == 0;
     const CUtensorMap tc = make_tmap_box(dz_all.data_ptr(), 2, cols, rows, 1, width, 0, 32, 64);
     launch_tiles<true>(h, w, at, cols, p, &tc, stream);
     const Tensor dz = dz_all.narrow(1, 0, cols), wp = w.narrow(0, at, cols);
-    if (direct) {
-      gemm_bf16_persistent(dz, wp, dh.narrow(1, 0, K), false, true, 1.0, false, err, -1);
-    } else if (want_dh) {
-      const int64_t here = slices == 1 ? cols : slice_cols, whole = slices == 1 ? 1 : std::min(slices, cols / here), rest = cols - whole * here;
-      if (whole)
-        gemm_bf16_persistent(dz_all.as_strided({whole, rows, here}, {here, width, 1}), wp.as_strided({whole, here, K}, {here * w.stride(0), w.stride(0), 1}, wp.storage_offset()),
-                             part.narrow(0, 0, whole).narrow(2, 0, K), false, true, 1.0, !first, err, -1);
-      // the columns behind the last whole slice: a slice of their own in a first piece, added to the first slice's sum where there is none for them
-      if (rest) {
-        const bool own = whole < slices;
-        gemm_bf16_persistent(dz.narrow(1, whole * here, rest), wp.narrow(0, whole * here, rest), part[own ? whole : 0].narrow(1, 0, K), false, true, 1.0, !(own && first), err, -1);
-      }
-    }
+    if (direct) gemm_bf16_scaled(dz, wp, dh.narrow(1, 0, K), false, true, num, den, false, 0, err);
+    else if (want_dh) gemm_bf16_scaled(dz, wp, part.narrow(2, 0, K), false, true, num, den, !first, slabs, err);
     if (want_dw) {
-      if (grad.has_value()) gemm_bf16_persistent(dz, h, grad->narrow(0, at, cols), true, true, 1.0, true, err, -1);
-      else gemm_bf16_persistent(dz, h, dw.narrow(0, at, cols).narrow(1, 0, K), true, true, 1.0, false, err, -1);
+      if (grad.has_value()) gemm_bf16_scaled(dz, h, grad->narrow(0, at, cols), true, true, num, den, true, 0, err);
+      else gemm_bf16_scaled(dz, h, dw.narrow(0, at, cols).narrow(1, 0, K), true, true, num, den, false, 0, err);
     }
   }
   if (want_dh && !direct) {
     dh = at::empty({rows, K}, fp32_dh ? f32 : hidden.options());
-    launch(vocab_slices_kernel, (unsigned)std::min<int64_t>((rows * K + 255) / 256, kNumSMs * 8), 256, 0, stream, (const float*)part.data_ptr<float>(), (int)slices, (long long)(rows * Kp),
-           (long long)rows, (int)K, (int)Kp, dh.data_ptr(), !fp32_dh);
+    auto kernel = fp32_dh ? vocab_slabs_kernel<false> : vocab_slabs_kernel<true>;
+    launch(kernel, (unsigned)std::min<int64_t>((rows + 7) / 8, kNumSMs * 8), 256, 0, stream, (const float*)part.data_ptr<float>(), (int)slabs, (long long)(rows * Kp), (int)rows, (int)K, (int)Kp,
+           dh.data_ptr());
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     count_launch();
-  } else if (direct && Kp != K) dh = dh.narrow(1, 0, K).contiguous();
-  if (dw.defined() && Kp != K) dw = dw.narrow(1, 0, K).contiguous();
+  } else if (direct && Kp != K) {
+    const Tensor wide = dh.narrow(1, 0, K);
+    dh = at::empty({rows, K}, wide.options());
+    copy_rows(wide, dh, stream);
+  }
+  if (dw.defined() && Kp != K) {
+    const Tensor wide = dw.narrow(1, 0, K);
+    dw = at::empty({vocab, K}, wide.options());
+    copy_rows(wide, dw, stream);
+  }
   return {dh, dw};
 }
 
