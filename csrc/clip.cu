@@ -9,18 +9,14 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <cuda_fp16.h>
 
 #include <algorithm>
 
-#include "common.cuh"
+#include "packs.cuh"
 #include "host.h"
 #include "launch.cuh"
 
 namespace q38 {
-
-template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
 enum ClipType : int { CLIP_F32 = 0, CLIP_BF16 = 1, CLIP_F16 = 2 };
 
@@ -48,24 +44,26 @@ __device__ __forceinline__ int clip_find(const ClipList<CAP>& l, int piece) {
   return lo;
 }
 
-template <typename T, int VEC> struct alignas(VEC * sizeof(T)) ClipPack { T v[VEC]; };
-
 template <typename T, int VEC>
 __device__ __forceinline__ void clip_squares(const T* in, int n, double (&acc)[4]) {
   constexpr int BATCH = VEC == 1 ? 8 : 4;
   const int packs = n / VEC;
+#pragma unroll 1
   for (int base = threadIdx.x; base < packs; base += CLIP_THREADS * BATCH) {
-    ClipPack<T, VEC> v[BATCH];
+    Pack<T, VEC> v[BATCH];
 #pragma unroll
     for (int j = 0; j < BATCH; ++j)
-      if (base + j * CLIP_THREADS < packs) v[j] = reinterpret_cast<const ClipPack<T, VEC>*>(in)[base + j * CLIP_THREADS];
+      if (base + j * CLIP_THREADS < packs) v[j] = load_pack<T, VEC>(in + (base + j * CLIP_THREADS) * VEC);
 #pragma unroll
     for (int j = 0; j < BATCH; ++j)
       if (base + j * CLIP_THREADS < packs) {
+        float f[VEC];
+        unpack(v[j], f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) { const double d = (double)to_float(v[j].v[e]); acc[(VEC == 1 ? j : e) & 3] += d * d; }
+        for (int e = 0; e < VEC; ++e) { const double d = (double)f[e]; acc[(VEC == 1 ? j : e) & 3] += d * d; }
       }
   }
+#pragma unroll 1
   for (int i = packs * VEC + threadIdx.x; i < n; i += CLIP_THREADS) { const double d = (double)to_float(in[i]); acc[0] += d * d; }
 }
 
@@ -73,19 +71,23 @@ template <typename T, int VEC>
 __device__ __forceinline__ void clip_scale(const T* in, T* out, int n, float factor) {
   constexpr int BATCH = VEC == 1 ? 8 : 4;
   const int packs = n / VEC;
+#pragma unroll 1
   for (int base = threadIdx.x; base < packs; base += CLIP_THREADS * BATCH) {
-    ClipPack<T, VEC> v[BATCH];
+    Pack<T, VEC> v[BATCH];
 #pragma unroll
     for (int j = 0; j < BATCH; ++j)
-      if (base + j * CLIP_THREADS < packs) v[j] = reinterpret_cast<const ClipPack<T, VEC>*>(in)[base + j * CLIP_THREADS];
+      if (base + j * CLIP_THREADS < packs) v[j] = load_pack<T, VEC>(in + (base + j * CLIP_THREADS) * VEC);
 #pragma unroll
     for (int j = 0; j < BATCH; ++j)
       if (base + j * CLIP_THREADS < packs) {
+        float f[VEC];
+        unpack(v[j], f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[j].v[e] = from_float<T>(to_float(v[j].v[e]) * factor);
-        reinterpret_cast<ClipPack<T, VEC>*>(out)[base + j * CLIP_THREADS] = v[j];
+        for (int e = 0; e < VEC; ++e) f[e] *= factor;
+        store_pack<T, VEC>(out + (base + j * CLIP_THREADS) * VEC, pack<T, VEC>(f));
       }
   }
+#pragma unroll 1
   for (int i = packs * VEC + threadIdx.x; i < n; i += CLIP_THREADS) out[i] = from_float<T>(to_float(in[i]) * factor);
 }
 
@@ -101,7 +103,7 @@ __device__ __forceinline__ void clip_scale(const T* in, T* out, int n, float fac
   }
 
 template <int CAP>
-__global__ void __launch_bounds__(CLIP_THREADS) clip_norm_kernel(const __grid_constant__ ClipList<CAP> l, double* __restrict__ partial) {
+__global__ void __launch_bounds__(CLIP_THREADS, 2) clip_norm_kernel(const __grid_constant__ ClipList<CAP> l, double* __restrict__ partial) {
   grid_wait();
   __shared__ double sums[CLIP_THREADS / 32];
   double acc[4] = {0.0, 0.0, 0.0, 0.0};
@@ -137,7 +139,7 @@ __device__ __forceinline__ double clip_total(const double* partial, int parts, d
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(CLIP_THREADS) clip_scale_kernel(const __grid_constant__ ClipList<CAP> l, const double* __restrict__ partial, int parts, float max_norm, float* norm) {
+__global__ void __launch_bounds__(CLIP_THREADS, 2) clip_scale_kernel(const __grid_constant__ ClipList<CAP> l, const double* __restrict__ partial, int parts, float max_norm, float* norm) {
   grid_wait();
   __shared__ double sums[CLIP_THREADS / 32];
   const float total = (float)clip_total(partial, parts, sums);
@@ -195,7 +197,7 @@ void run(at::TensorList grads, at::TensorList outs, int piece, double max_norm, 
   const auto lists = lists_of<CAP>(grads, outs, piece);
   int parts = 0;
   std::vector<int> grid;
-  for (const auto& l : lists) { grid.push_back(std::min(l.pieces, 4 * kNumSMs)); parts += grid.back(); }
+  for (const auto& l : lists) { grid.push_back(std::min(l.pieces, 2 * kNumSMs)); parts += grid.back(); }
   const Tensor partial = at::empty({std::max(parts, 1)}, norm.options().dtype(at::kDouble));
   double* sums = partial.data_ptr<double>();
   for (size_t i = 0, at = 0; i < lists.size(); at += grid[i++]) {

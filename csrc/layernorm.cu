@@ -12,43 +12,36 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <cuda_fp16.h>
 
-#include "common.cuh"
+#include "packs.cuh"
 #include "host.h"
 #include "launch.cuh"
 
 namespace q38 {
 
-template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-
-enum ParamType : int { PARAM_NONE = 0, PARAM_F32 = 1, PARAM_BF16 = 2, PARAM_F16 = 3 };
+enum ParamType : int { PARAM_F32 = 0, PARAM_BF16 = 1, PARAM_F16 = 2 };       // type of a weight's gradient
 
 struct LnArgs {
-  const void *x, *w, *b, *dy;
+  const void *x, *dy;
+  const float *w, *b;
   void* out;                       // y or dx
   float *mean, *rstd, *partial;    // [rows], [rows], [CTAs][2][dim]
   long long rows, ldx, lddy;
-  int dim, wt, bt, groups;         // groups of threads per CTA
+  int dim, groups;                 // groups of threads per CTA
   float eps;
 };
 
-template <typename T, int VEC> struct alignas(VEC * sizeof(T)) LnPack { T v[VEC]; };
-
-// VEC parameters at `at` in fp32; the type is one for the launch, so the branch is uniform
+// VEC parameters at `at`, or `none` where the layer has none
 template <int VEC>
-__device__ __forceinline__ void ln_param(const void* p, int type, int at, float (&out)[VEC], float none) {
-  if (type == PARAM_F32) {
-    const LnPack<float, VEC> v = reinterpret_cast<const LnPack<float, VEC>*>(reinterpret_cast<const float*>(p) + at)[0];
+__device__ __forceinline__ void ln_param(const float* p, int at, float (&out)[VEC], float none) {
+  if (p != nullptr) {
+    float part[VEC < 4 ? VEC : 4];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = v.v[i];
-  } else if (type == PARAM_BF16) {
+    for (int q = 0; q < VEC; q += 4) {                           // 16 bytes at a time
+      unpack(load_pack<float, VEC < 4 ? VEC : 4>(p + at + q), part);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[at + i]);
-  } else if (type == PARAM_F16) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[i] = __half2float(reinterpret_cast<const __half*>(p)[at + i]);
+      for (int i = 0; i < (VEC < 4 ? VEC : 4); ++i) out[q + i] = part[i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) out[i] = none;
@@ -76,7 +69,7 @@ __device__ __forceinline__ float2 ln_group_sum(float a, float b, float2* scratch
 }
 
 template <typename InT, typename OutT, int VEC, int E, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) layer_norm_fwd_kernel(LnArgs p) {
+__global__ void __launch_bounds__(WARP ? 256 : 1024, WARP ? (E > 16 ? 5 : 6) : 1) layer_norm_fwd_kernel(LnArgs p) {
   grid_wait();
   __shared__ float2 scratch[8][64];
   const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
@@ -85,52 +78,61 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) layer_norm_fwd_kernel(LnArg
   const InT* x = reinterpret_cast<const InT*>(p.x) + row * p.ldx;
   OutT* y = reinterpret_cast<OutT*>(p.out) + row * p.dim;
   int turn = 0;
-  float v[E];
+  Pack<InT, VEC> v[E / VEC];                                   // as they came: half the registers for 16-bit rows, so more of them are on their way
   float sum = 0.f;
 #pragma unroll
   for (int c = 0; c < E / VEC; ++c) {
     const int at = (c * G + t) * VEC;
-    if (at < p.dim) {
-      const LnPack<InT, VEC> in = *reinterpret_cast<const LnPack<InT, VEC>*>(x + at);
+    if (at < p.dim) v[c] = load_pack<InT, VEC>(x + at);
+  }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) { v[c * VEC + i] = to_float(in.v[i]); sum += v[c * VEC + i]; }
+  for (int c = 0; c < E / VEC; ++c) {
+    if ((c * G + t) * VEC < p.dim) {
+      float f[VEC];
+      unpack(v[c], f);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum += f[i];
     }
   }
-  const float mu = ln_group_sum<WARP>(sum, 0.f, scratch[WARP ? 0 : group], turn, G, group).x / p.dim;
+  const float inv = 1.f / p.dim;
+  const float mu = ln_group_sum<WARP>(sum, 0.f, scratch[WARP ? 0 : group], turn, G, group).x * inv;
   float ss = 0.f;
 #pragma unroll
   for (int c = 0; c < E / VEC; ++c) {
     if ((c * G + t) * VEC < p.dim) {
+      float f[VEC];
+      unpack(v[c], f);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) { v[c * VEC + i] -= mu; ss += v[c * VEC + i] * v[c * VEC + i]; }
+      for (int i = 0; i < VEC; ++i) { const float d = f[i] - mu; ss += d * d; }
     }
   }
-  const float r = rsqrtf(ln_group_sum<WARP>(ss, 0.f, scratch[WARP ? 0 : group], turn, G, group).x / p.dim + p.eps);
+  const float r = rsqrtf(ln_group_sum<WARP>(ss, 0.f, scratch[WARP ? 0 : group], turn, G, group).x * inv + p.eps);
   if (t == 0 && p.mean != nullptr) { p.mean[row] = mu; p.rstd[row] = r; }
 #pragma unroll
   for (int c = 0; c < E / VEC; ++c) {
     const int at = (c * G + t) * VEC;
     if (at < p.dim) {
-      float w[VEC], b[VEC];
-      ln_param<VEC>(p.w, p.wt, at, w, 1.f);
-      ln_param<VEC>(p.b, p.bt, at, b, 0.f);
-      LnPack<OutT, VEC> o;
+      float f[VEC], w[VEC], b[VEC];
+      unpack(v[c], f);
+      ln_param<VEC>(p.w, at, w, 1.f);
+      ln_param<VEC>(p.b, at, b, 0.f);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) o.v[i] = from_float<OutT>(v[c * VEC + i] * r * w[i] + b[i]);
-      *reinterpret_cast<LnPack<OutT, VEC>*>(y + at) = o;
+      for (int i = 0; i < VEC; ++i) f[i] = (f[i] - mu) * r * w[i] + b[i];
+      store_pack<OutT, VEC>(y + at, pack<OutT, VEC>(f));
     }
   }
 }
 
 // ACC: where the weight sums of a thread's columns live (registers, or shared memory for rows so long that registers would spill; each cell has one owner).
 template <typename InT, typename OutT, int VEC, int E, bool WARP, bool ACC_SMEM>
-__global__ void __launch_bounds__(ACC_SMEM ? 1024 : 512, 1) layer_norm_bwd_kernel(LnArgs p) {
+__global__ void __launch_bounds__(ACC_SMEM ? 1024 : 512, E == 8 && VEC == 8 ? 2 : 1) layer_norm_bwd_kernel(LnArgs p) {
   grid_wait();
   extern __shared__ float sums[];                                // [2][dim]
   __shared__ float2 scratch[16][64];
   constexpr int N = E / VEC;
   const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
   const bool wanted = p.partial != nullptr;
+  const float inv = 1.f / p.dim;
   float aw[ACC_SMEM ? 1 : E], ab[ACC_SMEM ? 1 : E];
   if constexpr (ACC_SMEM) {
     for (int i = threadIdx.x; i < 2 * p.dim; i += blockDim.x) sums[i] = 0.f;
@@ -141,61 +143,68 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : 512, 1) layer_norm_bwd_kerne
   }
   const long long stride = (long long)gridDim.x * p.groups;
   long long row = (long long)blockIdx.x * p.groups + group;
-  LnPack<InT, VEC> nx[N];
-  LnPack<OutT, VEC> nd[N];
-  float nmu = 0.f, nr = 0.f;
+  constexpr bool AHEAD = !ACC_SMEM;                              // with 1024 threads there are no registers for a row ahead
+  Pack<InT, VEC> x[N], nx[N];
+  Pack<OutT, VEC> d[N], nd[N];
+  float mu = 0.f, r = 0.f, nmu = 0.f, nr = 0.f;
   auto fetch = [&](long long at_row) {
     if (at_row >= p.rows) return;
-    const InT* x = reinterpret_cast<const InT*>(p.x) + at_row * p.ldx;
-    const OutT* d = reinterpret_cast<const OutT*>(p.dy) + at_row * p.lddy;
+    const InT* px = reinterpret_cast<const InT*>(p.x) + at_row * p.ldx;
+    const OutT* pd = reinterpret_cast<const OutT*>(p.dy) + at_row * p.lddy;
     nmu = p.mean[at_row]; nr = p.rstd[at_row];
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       const int at = (c * G + t) * VEC;
       if (at < p.dim) {
-        nx[c] = *reinterpret_cast<const LnPack<InT, VEC>*>(x + at);
-        nd[c] = *reinterpret_cast<const LnPack<OutT, VEC>*>(d + at);
+        nx[c] = load_pack<InT, VEC>(px + at);
+        nd[c] = load_pack<OutT, VEC>(pd + at);
       }
     }
   };
-  if (!ACC_SMEM) fetch(row);
+  if (AHEAD) fetch(row);
   int turn = 0;
+#pragma unroll 1
   for (; row < p.rows; row += stride) {
-    if (ACC_SMEM) fetch(row);                                    // 64 registers per thread: none for a row ahead
-    float hat[E], g[E];
-    const float mu = nmu, r = nr;
+    if (!AHEAD) fetch(row);
+#pragma unroll
+    for (int c = 0; c < N; ++c) { x[c] = nx[c]; d[c] = nd[c]; }
+    mu = nmu; r = nr;
+    if (AHEAD) fetch(row + stride);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
       const int at = (c * G + t) * VEC;
       if (at < p.dim) {
-        float w[VEC];
-        ln_param<VEC>(p.w, p.wt, at, w, 1.f);
+        float xv[VEC], dv[VEC], w[VEC];
+        unpack(x[c], xv);
+        unpack(d[c], dv);
+        ln_param<VEC>(p.w, at, w, 1.f);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           const int e = c * VEC + i;
-          const float d = to_float(nd[c].v[i]);
-          hat[e] = (to_float(nx[c].v[i]) - mu) * r;
-          if constexpr (ACC_SMEM) { sums[at + i] += d * hat[e]; sums[p.dim + at + i] += d; }
-          else { aw[e] += d * hat[e]; ab[e] += d; }
-          g[e] = d * w[i];
-          s1 += g[e]; s2 += g[e] * hat[e];
+          const float hat = (xv[i] - mu) * r, g = dv[i] * w[i];
+          if constexpr (ACC_SMEM) { sums[at + i] += dv[i] * hat; sums[p.dim + at + i] += dv[i]; }
+          else { aw[e] += dv[i] * hat; ab[e] += dv[i]; }
+          s1 += g; s2 += g * hat;
         }
       }
     }
-    if (!ACC_SMEM) fetch(row + stride);
     const float2 s = ln_group_sum<WARP>(s1, s2, scratch[WARP ? 0 : group], turn, G, group);
-    if (p.out == nullptr) continue;
-    const float m1 = s.x / p.dim, m2 = s.y / p.dim;
-    InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
+    if (p.out != nullptr) {
+      const float m1 = s.x * inv, m2 = s.y * inv;
+      InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      const int at = (c * G + t) * VEC;
-      if (at < p.dim) {
-        LnPack<InT, VEC> o;
+      for (int c = 0; c < N; ++c) {                              // from the packed row again: the values themselves would take twice its registers
+        const int at = (c * G + t) * VEC;
+        if (at < p.dim) {
+          float xv[VEC], dv[VEC], w[VEC];
+          unpack(x[c], xv);
+          unpack(d[c], dv);
+          ln_param<VEC>(p.w, at, w, 1.f);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o.v[i] = from_float<InT>(r * (g[c * VEC + i] - m1 - hat[c * VEC + i] * m2));
-        *reinterpret_cast<LnPack<InT, VEC>*>(dx + at) = o;
+          for (int i = 0; i < VEC; ++i) xv[i] = r * (dv[i] * w[i] - m1 - (xv[i] - mu) * r * m2);
+          store_pack<InT, VEC>(dx + at, pack<InT, VEC>(xv));
+        }
       }
     }
   }
@@ -240,8 +249,8 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(LnArgs p, bool ba
       if (threadIdx.x == 0 && p.mean != nullptr) { p.mean[row] = mu; p.rstd[row] = r; }
       OutT* y = reinterpret_cast<OutT*>(p.out) + row * p.dim;
       for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
-        ln_param<1>(p.w, p.wt, i, w, 1.f);
-        ln_param<1>(p.b, p.bt, i, b, 0.f);
+        ln_param<1>(p.w, i, w, 1.f);
+        ln_param<1>(p.b, i, b, 0.f);
         y[i] = from_float<OutT>((to_float(x[i]) - mu) * r * w[0] + b[0]);
       }
     } else {
@@ -249,7 +258,7 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(LnArgs p, bool ba
       const float mu = p.mean[row], r = p.rstd[row];
       float s1 = 0.f, s2 = 0.f;
       for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
-        ln_param<1>(p.w, p.wt, i, w, 1.f);
+        ln_param<1>(p.w, i, w, 1.f);
         const float d = to_float(dy[i]), hat = (to_float(x[i]) - mu) * r;
         s1 += d * w[0]; s2 += d * w[0] * hat;
         if (mine != nullptr) { mine[i] += d * hat; mine[p.dim + i] += d; }
@@ -258,42 +267,49 @@ __global__ void __launch_bounds__(1024) layer_norm_long_kernel(LnArgs p, bool ba
       if (p.out == nullptr) continue;
       InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
       for (int i = threadIdx.x; i < p.dim; i += blockDim.x) {
-        ln_param<1>(p.w, p.wt, i, w, 1.f);
+        ln_param<1>(p.w, i, w, 1.f);
         dx[i] = from_float<InT>(r * (to_float(dy[i]) * w[0] - m1 - (to_float(x[i]) - mu) * r * m2));
       }
     }
   }
 }
 
-// dw and db from the CTAs' parts: 32 columns per CTA, sixteen threads per column in strides of sixteen parts, then in order.
-__global__ void __launch_bounds__(512) layer_norm_sums_kernel(const float* __restrict__ partial, int parts, int dim, void* dw, int wt, void* db, int bt) {
+// dw and db from the CTAs' parts: 32 columns per CTA, 32 threads per column in strides of 32 parts (four reads in flight), then in order.
+__global__ void __launch_bounds__(1024) layer_norm_sums_kernel(const float* __restrict__ partial, int parts, int dim, void* dw, int wt, void* db, int bt) {
   grid_wait();
-  __shared__ float acc[16][33];
+  __shared__ float acc[32][33];
   const int col = blockIdx.x * 32 + threadIdx.x, which = blockIdx.y;
+  void* to = which ? db : dw;
+  if (to == nullptr) return;
   float s = 0.f;
-  if (col < dim)
-    for (int q = threadIdx.y; q < parts; q += 16) s += partial[((long long)q * 2 + which) * dim + col];
+  if (col < dim) {
+    const float* in = partial + (long long)which * dim + col;
+    const long long step = 2ll * dim;
+    for (int q = threadIdx.y; q < parts; q += 128) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = q + 32 * e < parts ? in[(q + 32 * e) * step] : 0.f;
+      s += (v[0] + v[1]) + (v[2] + v[3]);
+    }
+  }
   acc[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y != 0 || col >= dim) return;
-  s = 0.f;
-#pragma unroll
-  for (int q = 0; q < 16; ++q) s += acc[q][threadIdx.x];
-  void* to = which ? db : dw;
-  const int type = which ? bt : wt;
-  if (to == nullptr) return;
-  if (type == PARAM_F32) reinterpret_cast<float*>(to)[col] = s;
-  else if (type == PARAM_BF16) reinterpret_cast<__nv_bfloat16*>(to)[col] = __float2bfloat16_rn(s);
-  else reinterpret_cast<__half*>(to)[col] = __float2half_rn(s);
+  s = warp_sum(acc[threadIdx.x][threadIdx.y]);                   // a warp per column from here
+  const int mine = blockIdx.x * 32 + threadIdx.y, type = which ? bt : wt;
+  if (threadIdx.x != 0 || mine >= dim) return;
+  if (type == PARAM_F32) reinterpret_cast<float*>(to)[mine] = s;
+  else if (type == PARAM_BF16) reinterpret_cast<__nv_bfloat16*>(to)[mine] = __float2bfloat16_rn(s);
+  else reinterpret_cast<__half*>(to)[mine] = __float2half_rn(s);
 }
 
 namespace {
 
 int param_type(const c10::optional<at::Tensor>& t) {
-  if (!t.has_value()) return PARAM_NONE;
-  return t->scalar_type() == at::kFloat ? PARAM_F32 : t->scalar_type() == at::kBFloat16 ? PARAM_BF16 : PARAM_F16;
+  return !t.has_value() || t->scalar_type() == at::kFloat ? PARAM_F32 : t->scalar_type() == at::kBFloat16 ? PARAM_BF16 : PARAM_F16;
 }
-const void* param_ptr(const c10::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
+// Parameters as the kernels take them: fp32 (a vector in another type is converted, which costs a small launch and no branch in the kernels)
+at::Tensor param(const c10::optional<at::Tensor>& t) { return t.has_value() ? t->to(at::kFloat).contiguous() : at::Tensor(); }
+const float* param_ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 constexpr int LN_LONGEST = 16384;          // longest row that a CTA of 1024 threads holds in registers
@@ -329,12 +345,16 @@ void launch_fwd(LnArgs& p, cudaStream_t stream) {
 }
 
 struct BwdShape { int G, groups, ctas; };
-BwdShape bwd_shape(long long rows, int dim) {
-  BwdShape s;
+// Threads per row, rows per CTA and CTAs.  Eight 16-bit elements per thread take 64 registers (1024 threads per SM), eight others up to 96 (640), sixteen up to 128 (512);
+// what counts is the bytes on their way, 32 to 64 KB per SM in each case.  As many CTAs as are resident at once.
+BwdShape bwd_shape(long long rows, int dim, bool packed16) {
   if (dim > LN_LONGEST) return {1024, 1, (int)std::min<long long>(rows, kNumSMs)};
+  BwdShape s;
+  const bool eight = dim <= 256 || (dim > 512 && dim <= 4096);
+  const int threads = eight && !packed16 ? 320 : 512, resident = eight ? (packed16 ? 1024 : 640) : 512;
   s.G = dim <= 512 ? 32 : group_of(dim, dim <= 4096 ? 8 : 16);
-  s.groups = std::max(1, 512 / s.G);
-  s.ctas = (int)std::min<long long>((rows + s.groups - 1) / s.groups, (s.G * s.groups > 512 ? 1 : 2) * kNumSMs);
+  s.groups = std::max(1, threads / s.G);
+  s.ctas = (int)std::min<long long>((rows + s.groups - 1) / s.groups, std::max(1, resident / (s.G * s.groups)) * kNumSMs);
   return s;
 }
 
@@ -356,9 +376,9 @@ void launch_bwd(LnArgs& p, const BwdShape& s, cudaStream_t stream) {
 void check_params(const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b) {
   for (const auto* t : {&w, &b})
     if (t->has_value())
-      TORCH_CHECK((*t)->device() == x.device() && (*t)->dim() == 1 && (*t)->size(0) == x.size(1) && (*t)->is_contiguous() &&
+      TORCH_CHECK((*t)->device() == x.device() && (*t)->dim() == 1 && (*t)->size(0) == x.size(1) &&
                   ((*t)->scalar_type() == at::kFloat || (*t)->scalar_type() == at::kBFloat16 || (*t)->scalar_type() == at::kHalf),
-                  "layer_norm: weight and bias are contiguous fp32, bf16 or fp16 vectors of the last dimension's length on the input's device");
+                  "layer_norm: weight and bias are fp32, bf16 or fp16 vectors of the last dimension's length on the input's device");
 }
 
 }  // namespace
@@ -373,7 +393,8 @@ std::vector<at::Tensor> layer_norm_fwd(const at::Tensor& x, const c10::optional<
   auto y = at::empty({p.rows, p.dim}, x.options().dtype(out_type));
   auto stats = at::empty({save ? 2 : 0, p.rows}, x.options().dtype(at::kFloat));
   auto mean = save ? stats[0] : stats, rstd = save ? stats[1] : stats;
-  p.x = x.data_ptr(); p.out = y.data_ptr(); p.w = param_ptr(w); p.b = param_ptr(b); p.wt = param_type(w); p.bt = param_type(b);
+  const at::Tensor wf = param(w), bf = param(b);
+  p.x = x.data_ptr(); p.out = y.data_ptr(); p.w = param_ptr(wf); p.b = param_ptr(bf);
   if (save) { p.mean = mean.data_ptr<float>(); p.rstd = rstd.data_ptr<float>(); }
   by_type(x.scalar_type(), out_type, [&](auto in, auto out) {
     using InT = decltype(in);
@@ -408,18 +429,20 @@ std::vector<at::Tensor> layer_norm_bwd(const at::Tensor& dy, const at::Tensor& x
     if (want_db) db.zero_();
     return {dx, dw, db};
   }
-  const BwdShape s = bwd_shape(p.rows, p.dim);
+  const int per16 = 16 / (int)x.element_size();
+  const at::Tensor wf = param(w);
+  p.x = x.data_ptr(); p.dy = dy.data_ptr(); p.w = param_ptr(wf);
+  p.out = want_dx ? dx.data_ptr() : nullptr;
+  const bool vec = p.dim % per16 == 0 && p.ldx % per16 == 0 && p.lddy % per16 == 0 && on16(p.x) && on16(p.dy) && on16(p.out) && on16(p.w);
+  const BwdShape s = bwd_shape(p.rows, p.dim, vec && per16 == 8);
   at::Tensor partial;
   if (want_dw || want_db) partial = at::empty({s.ctas, 2, p.dim}, x.options().dtype(at::kFloat));
-  p.x = x.data_ptr(); p.dy = dy.data_ptr(); p.w = param_ptr(w); p.wt = param_type(w);
-  p.out = want_dx ? dx.data_ptr() : nullptr;
   p.mean = mean.data_ptr<float>(); p.rstd = rstd.data_ptr<float>(); p.partial = partial.defined() ? partial.data_ptr<float>() : nullptr;
   auto stream = at::cuda::getCurrentCUDAStream();
   by_type(x.scalar_type(), dy.scalar_type(), [&](auto in, auto out) {
     using InT = decltype(in);
     using OutT = decltype(out);
     constexpr int VEC = 16 / sizeof(InT);
-    const bool vec = p.dim % VEC == 0 && p.ldx % VEC == 0 && p.lddy % VEC == 0 && on16(p.x) && on16(p.dy) && on16(p.out) && on16(p.w);
     if (p.dim > LN_LONGEST) launch(layer_norm_long_kernel<InT, OutT>, (unsigned)s.ctas, 1024, 0, stream, p, true);
     else if (vec) launch_bwd<InT, OutT, VEC>(p, s, stream);
     else launch_bwd<InT, OutT, 1>(p, s, stream);
@@ -427,7 +450,7 @@ std::vector<at::Tensor> layer_norm_bwd(const at::Tensor& dy, const at::Tensor& x
     count_launch();
   });
   if (partial.defined()) {
-    launch(layer_norm_sums_kernel, dim3((p.dim + 31) / 32, 2), dim3(32, 16), 0, stream, (const float*)p.partial, s.ctas, p.dim, want_dw ? dw.data_ptr() : nullptr,
+    launch(layer_norm_sums_kernel, dim3((p.dim + 31) / 32, 2), dim3(32, 32), 0, stream, (const float*)p.partial, s.ctas, p.dim, want_dw ? dw.data_ptr() : nullptr,
            param_type(w), want_db ? db.data_ptr() : nullptr, param_type(b));
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     count_launch();

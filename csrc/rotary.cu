@@ -12,47 +12,59 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <cuda_fp16.h>
 
-#include "common.cuh"
+#include "packs.cuh"
 #include "host.h"
 #include "launch.cuh"
 
 namespace q38 {
 
-template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+// Quotients by a number that is fixed for the launch: two multiplications, exact for any 32-bit dividend
+struct Divisor {
+  uint64_t inverse;                // floor(2^64 / d) + 1, or 0 for d = 1
+  uint32_t d;
+};
+__device__ __forceinline__ int quotient(int n, const Divisor& by) {
+  const uint64_t low = (uint64_t)(uint32_t)n * (uint32_t)by.inverse, high = (uint64_t)(uint32_t)n * (uint32_t)(by.inverse >> 32) + (low >> 32);
+  return by.d == 1 ? n : (int)(high >> 32);
+}
 
-struct RotarySide {               // queries or keys: strides of batch, token and head
+struct RotarySide {                // queries or keys: strides of batch, token and head
   const void* in;
   void* out;
   long long in_b, in_s, in_h, out_b, out_s, out_h;
 };
 struct RotaryArgs {
   RotarySide q, k;
-  const double* freq;             // [r / 2]
-  const void* pos;                // [batch or 1, tokens], 32 or 64 bits
-  long long pos_b, pos_s, tokens; // tokens = batch * seq
-  int seq, q_heads, heads, dim, half, units, per_cta, pos64;      // heads of both sides; units per head
+  const double* freq;              // [r / 2]
+  const void* pos;                 // [batch or 1, tokens], 32 or 64 bits
+  long long pos_b, pos_s, tokens;  // tokens = batch * seq
+  Divisor units, heads, half;      // units per head; heads of both sides; pairs per head
+  int seq, q_heads, dim, per_cta, pos64;
   float magnitude, sign;
 };
 
-constexpr int ROT_THREADS = 256, ROT_BATCH = 4;
-
-template <typename T, int VEC> struct alignas(VEC * sizeof(T)) RotPack { T v[VEC]; };
+constexpr int ROT_THREADS = 256, ROT_BATCH = 2, ROT_TOKENS = 64;
 
 // VEC == 1: a unit is one pair, or one element that passes through.  VEC > 1: two packs: one of each half, two neighbours of an interleaved head, or two
 // (the last unit perhaps one) that pass through.
 template <typename T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotaryArgs p) {
+__global__ void __launch_bounds__(ROT_THREADS, 5) rotary_kernel(const __grid_constant__ RotaryArgs p) {
   grid_wait();
   extern __shared__ float2 turns[];                      // [per_cta][half]: cos, sin
+  __shared__ long long base_of[ROT_TOKENS][4];           // where a token's queries and keys begin, in and out
   const long long first = (long long)blockIdx.x * p.per_cta;
-  const int count = (int)min((long long)p.per_cta, p.tokens - first);
-  for (int i = threadIdx.x; i < count * p.half; i += ROT_THREADS) {
-    const int local = i / p.half, f = i - local * p.half;
-    const long long token = first + local, b = token / p.seq, s = token - b * p.seq;
-    const long long at = b * p.pos_b + s * p.pos_s;
+  const int count = (int)min((long long)p.per_cta, p.tokens - first), half = p.half.d;
+  if (threadIdx.x < count) {
+    const long long token = first + threadIdx.x, b = token / p.seq, s = token - b * p.seq;
+    base_of[threadIdx.x][0] = b * p.q.in_b + s * p.q.in_s;
+    base_of[threadIdx.x][1] = b * p.q.out_b + s * p.q.out_s;
+    base_of[threadIdx.x][2] = b * p.k.in_b + s * p.k.in_s;
+    base_of[threadIdx.x][3] = b * p.k.out_b + s * p.k.out_s;
+  }
+  for (int i = threadIdx.x; i < count * half; i += ROT_THREADS) {
+    const int local = quotient(i, p.half), f = i - local * half;
+    const long long token = first + local, b = p.pos_b ? token / p.seq : 0, at = p.pos_b ? b * p.pos_b + (token - b * p.seq) * p.pos_s : token % p.seq * p.pos_s;
     const double t = p.pos64 ? (double)reinterpret_cast<const long long*>(p.pos)[at] : (double)reinterpret_cast<const int*>(p.pos)[at];
     const double turn = t * (p.freq[f] * 0.15915494309189533576888);            // 1 / (2 pi)
     float sn, cs;
@@ -61,57 +73,60 @@ __global__ void __launch_bounds__(ROT_THREADS) rotary_kernel(RotaryArgs p) {
   }
   __syncthreads();
 
-  constexpr int PACKS = 2;
-  const int rot_units = VEC == 1 ? p.half : p.half / VEC;
-  const int total = count * p.heads * p.units;
+  const int rot_units = VEC == 1 ? half : half / VEC, units = p.units.d, heads = p.heads.d;
+  const int total = count * heads * units;
   for (int base = threadIdx.x; base < total; base += ROT_THREADS * ROT_BATCH) {
-    RotPack<T, VEC> v[ROT_BATCH][PACKS];
-    const T* src[ROT_BATCH];
+    Pack<T, VEC> v[ROT_BATCH][2];
     T* dst[ROT_BATCH];
     int second[ROT_BATCH], angle[ROT_BATCH];             // distance of the second pack (0: there is none); first angle, or -1 where elements pass through
 #pragma unroll
     for (int j = 0; j < ROT_BATCH; ++j) {
       const int i = base + j * ROT_THREADS;
-      src[j] = nullptr;
+      dst[j] = nullptr;
       if (i < total) {
-        const int row = i / p.units, unit = i - row * p.units, local = row / p.heads, head = row - local * p.heads;
-        const long long token = first + local, b = token / p.seq, s = token - b * p.seq;
-        const bool key = head >= p.q_heads;
-        const RotarySide& side = key ? p.k : p.q;
-        const int h = key ? head - p.q_heads : head;
+        const int row = quotient(i, p.units), unit = i - row * units, local = quotient(row, p.heads), head = row - local * heads;
         int at;
         if (unit < rot_units) {
           at = INTERLEAVED ? 2 * VEC * unit : VEC * unit;
-          second[j] = INTERLEAVED ? VEC : p.half;
-          angle[j] = local * p.half + unit * VEC;
+          second[j] = INTERLEAVED ? VEC : half;
+          angle[j] = local * half + unit * VEC;
         } else {
           const int rest = unit - rot_units;
-          at = 2 * p.half + (VEC == 1 ? rest : 2 * VEC * rest);
+          at = 2 * half + (VEC == 1 ? rest : 2 * VEC * rest);
           second[j] = VEC > 1 && at + VEC < p.dim ? VEC : 0;
           angle[j] = -1;
         }
-        src[j] = reinterpret_cast<const T*>(side.in) + b * side.in_b + s * side.in_s + h * side.in_h + at;
-        dst[j] = reinterpret_cast<T*>(side.out) + b * side.out_b + s * side.out_s + h * side.out_h + at;
-        v[j][0] = *reinterpret_cast<const RotPack<T, VEC>*>(src[j]);
-        if (second[j]) v[j][1] = *reinterpret_cast<const RotPack<T, VEC>*>(src[j] + second[j]);
+        const bool key = head >= p.q_heads;
+        const RotarySide& side = key ? p.k : p.q;
+        const int h = key ? head - p.q_heads : head;
+        const T* src = reinterpret_cast<const T*>(side.in) + base_of[local][key ? 2 : 0] + h * side.in_h + at;
+        dst[j] = reinterpret_cast<T*>(side.out) + base_of[local][key ? 3 : 1] + h * side.out_h + at;
+        v[j][0] = load_pack<T, VEC>(src);
+        if (second[j]) v[j][1] = load_pack<T, VEC>(src + second[j]);
       }
     }
 #pragma unroll
     for (int j = 0; j < ROT_BATCH; ++j) {
-      if (src[j] == nullptr) continue;
-      if (angle[j] >= 0) {
+      if (dst[j] != nullptr) {
+        if (angle[j] >= 0) {
+          float f[2][VEC];
+          unpack(v[j][0], f[0]);
+          unpack(v[j][1], f[1]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float2 cs = turns[angle[j] + e];
-          T& lo = INTERLEAVED && VEC > 1 ? v[j][2 * e / VEC].v[2 * e % VEC] : v[j][0].v[e];
-          T& hi = INTERLEAVED && VEC > 1 ? v[j][(2 * e + 1) / VEC].v[(2 * e + 1) % VEC] : v[j][1].v[e];
-          const float a = to_float(lo), b = to_float(hi);
-          lo = from_float<T>(a * cs.x - b * cs.y);
-          hi = from_float<T>(b * cs.x + a * cs.y);
+          for (int e = 0; e < VEC; ++e) {
+            const float2 cs = turns[angle[j] + e];
+            float& lo = INTERLEAVED && VEC > 1 ? f[2 * e / VEC][2 * e % VEC] : f[0][e];
+            float& hi = INTERLEAVED && VEC > 1 ? f[(2 * e + 1) / VEC][(2 * e + 1) % VEC] : f[1][e];
+            const float a = lo, b = hi;
+            lo = a * cs.x - b * cs.y;
+            hi = b * cs.x + a * cs.y;
+          }
+          v[j][0] = pack<T, VEC>(f[0]);
+          v[j][1] = pack<T, VEC>(f[1]);
         }
+        store_pack<T, VEC>(dst[j], v[j][0]);
+        if (second[j]) store_pack<T, VEC>(dst[j] + second[j], v[j][1]);
       }
-      *reinterpret_cast<RotPack<T, VEC>*>(dst[j]) = v[j][0];
-      if (second[j]) *reinterpret_cast<RotPack<T, VEC>*>(dst[j] + second[j]) = v[j][1];
     }
   }
 }
@@ -129,21 +144,23 @@ bool packs_fit(const Tensor& t, int vec) {
   return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && t.stride(0) % vec == 0 && t.stride(1) % vec == 0 && t.stride(2) % vec == 0;
 }
 
+Divisor divisor(int d) { return {d > 1 ? ~0ull / d + 1 : 0, (uint32_t)d}; }
+
 template <typename T>
 void launch_rotary(RotaryArgs& p, bool fit, bool interleaved, cudaStream_t stream) {
   constexpr int VEC = 16 / sizeof(T);
-  const int rest = p.dim - 2 * p.half;
-  const bool vec = fit && p.dim % VEC == 0 && p.half % VEC == 0;
-  p.units = vec ? p.half / VEC + (rest / VEC + 1) / 2 : p.half + rest;
-  // Tokens per CTA: eight units per thread (two batches of loads), fewer where that leaves an SM without work; their angles fit 32 KB
-  const long long per_token = (long long)p.heads * p.units;
-  long long n = std::max<long long>(1, 8 * ROT_THREADS / per_token);
+  const int half = (int)p.half.d, rest = p.dim - 2 * half;
+  const bool vec = fit && p.dim % VEC == 0 && half % VEC == 0;
+  p.units = divisor(vec ? half / VEC + (rest / VEC + 1) / 2 : half + rest);
+  // Tokens per CTA: eight units per thread, fewer where that leaves an SM without work; their angles fit 32 KB
+  const long long per_token = (long long)p.heads.d * p.units.d;
+  long long n = std::min<long long>(ROT_TOKENS, std::max<long long>(1, 8 * ROT_THREADS / per_token));
   n = std::min(n, std::max<long long>(1, p.tokens / (2 * kNumSMs)));
-  if (p.half) n = std::max<long long>(1, std::min<long long>(n, 4096 / p.half));
+  if (half) n = std::max<long long>(1, std::min<long long>(n, 4096 / half));
   p.per_cta = (int)n;
   const long long grid = (p.tokens + n - 1) / n;
   TORCH_CHECK(grid < (1ll << 31) && per_token * n < (1ll << 30), "rotary: tensor too large");
-  const size_t smem = size_t(p.per_cta) * p.half * sizeof(float2);
+  const size_t smem = size_t(p.per_cta) * half * sizeof(float2);
   auto go = [&](auto kernel) {
     if (smem > 48 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     launch(kernel, (unsigned)grid, ROT_THREADS, smem, stream, p);
@@ -169,12 +186,12 @@ std::pair<Tensor, Tensor> rotary_apply(const Tensor& q_in, const Tensor& k_in, c
   if (q.defined()) { p.q = side_of(q, qo); fit = fit && packs_fit(q, vec) && packs_fit(qo, vec); }
   if (k.defined()) { p.k = side_of(k, ko); fit = fit && packs_fit(k, vec) && packs_fit(ko, vec); }
   p.q_heads = q.defined() ? (int)q.size(2) : 0;
-  p.heads = p.q_heads + (k.defined() ? (int)k.size(2) : 0);
-  p.seq = (int)any.size(1); p.tokens = any.size(0) * any.size(1); p.dim = (int)any.size(3); p.half = (int)freq.size(0);
+  p.heads = divisor(p.q_heads + (k.defined() ? (int)k.size(2) : 0));
+  p.seq = (int)any.size(1); p.tokens = any.size(0) * any.size(1); p.dim = (int)any.size(3); p.half = divisor((int)freq.size(0));
   p.freq = freq.data_ptr<double>(); p.pos = pos.data_ptr(); p.pos64 = pos.scalar_type() == at::kLong;
   p.pos_b = pos.dim() == 2 && pos.size(0) > 1 ? pos.stride(0) : 0; p.pos_s = pos.stride(-1);
   p.magnitude = (float)magnitude; p.sign = (float)sign;
-  if (p.tokens > 0 && p.heads > 0) {
+  if (p.tokens > 0 && p.heads.d > 0) {
     auto stream = at::cuda::getCurrentCUDAStream();
     if (any.scalar_type() == at::kBFloat16) launch_rotary<__nv_bfloat16>(p, fit, interleaved, stream);
     else if (any.scalar_type() == at::kHalf) launch_rotary<__half>(p, fit, interleaved, stream);

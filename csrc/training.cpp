@@ -21,7 +21,6 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
-OptTensor dense(const OptTensor& t) { return t.has_value() ? OptTensor(t->contiguous()) : t; }
 bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 
 // ---- layer norm ---------------------------------------------------------------------------------------------------------------
@@ -33,14 +32,14 @@ Tensor as_rows(const Tensor& x) {
 
 struct LayerNorm : public torch::autograd::Function<LayerNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, at::ScalarType out_type) {
-    auto out = layer_norm_fwd(as_rows(x), dense(w), dense(b), eps, out_type, true);
+    auto out = layer_norm_fwd(as_rows(x), w, b, eps, out_type, true);
     ctx->save_for_backward({x, w.value_or(Tensor()), b.value_or(Tensor()), out[1], out[2]});
     return out[0].view(x.sizes());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm: a gradient of the gradient is not available");
     auto saved = ctx->get_saved_variables();
-    const OptTensor w = dense(optional_of(saved[1])), b = dense(optional_of(saved[2]));
+    const OptTensor w = optional_of(saved[1]), b = optional_of(saved[2]);
     const size_t b_edge = w.has_value() ? 2 : 1;                   // edges are counted over the tensors that were given
     auto out = layer_norm_bwd(as_rows(grads[0]), as_rows(saved[0]), w, b, saved[3], saved[4], ctx->needs_input_grad(0), w.has_value() && ctx->needs_input_grad(1),
                               b.has_value() && ctx->needs_input_grad(b_edge));
@@ -52,7 +51,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, doubl
   TORCH_CHECK(x.dim() > 0 && x.size(-1) > 0, "layer_norm: an input with a last dimension that is not empty required");
   const at::ScalarType to = out_type.value_or(x.scalar_type());
   if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(w) || wants_grad(b))) return LayerNorm::apply(x, w, b, eps, to);
-  return layer_norm_fwd(as_rows(x), dense(w), dense(b), eps, to, false)[0].view(x.sizes());
+  return layer_norm_fwd(as_rows(x), w, b, eps, to, false)[0].view(x.sizes());
 }
 
 // ---- rotary positions ------------------------------------------------------------------------------------------------------------
