@@ -44,24 +44,54 @@ __device__ __forceinline__ int clip_find(const ClipList<CAP>& l, int piece) {
   return lo;
 }
 
+// Squares of four 16-bit values one by one in 64 bits
+template <typename T>
+__device__ __noinline__ double clip_apart(uint32_t w0, uint32_t w1) {
+  Pack<T, 4> p;
+  p.w[0] = w0; p.w[1] = w1;
+  float f[4];
+  unpack(p, f);
+  double s = 0.0;
+#pragma unroll 1
+  for (int e = 0; e < 4; ++e) { const double d = (double)(e == 0 ? f[0] : e == 1 ? f[1] : e == 2 ? f[2] : f[3]); s += d * d; }
+  return s;
+}
+
+// Four 16-bit values: their squares are exact in fp32, and the sum of four has two roundings on a way, so one conversion to 64 bits does for four
+// (conversions run at an eighth of the fp32 rate).  bf16 has fp32's range: a sum that is near its ends, zeros aside, is taken apart.
+template <typename T>
+__device__ __forceinline__ double clip_four(uint32_t w0, uint32_t w1) {
+  Pack<T, 4> p;
+  p.w[0] = w0; p.w[1] = w1;
+  float f[4];
+  unpack(p, f);
+  const float s = fmaf(f[0], f[0], f[1] * f[1]) + fmaf(f[2], f[2], f[3] * f[3]);
+  if (s < 1e-28f || s > 1e38f) return ((w0 | w1) & 0x7fff7fffu) == 0u ? 0.0 : clip_apart<T>(w0, w1);
+  return (double)s;
+}
+
 template <typename T, int VEC>
-__device__ __forceinline__ void clip_squares(const T* in, int n, double (&acc)[4]) {
-  constexpr int BATCH = VEC == 1 ? 8 : 4;
+__device__ __forceinline__ void clip_squares(const T* in, int n, double (&acc)[2]) {
+  constexpr int BATCH = 4;
   const int packs = n / VEC;
 #pragma unroll 1
   for (int base = threadIdx.x; base < packs; base += CLIP_THREADS * BATCH) {
-    Pack<T, VEC> v[BATCH];
+    Pack<T, VEC> v[BATCH] = {};                                  // zeros behind the end
 #pragma unroll
     for (int j = 0; j < BATCH; ++j)
       if (base + j * CLIP_THREADS < packs) v[j] = load_pack<T, VEC>(in + (base + j * CLIP_THREADS) * VEC);
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j)
-      if (base + j * CLIP_THREADS < packs) {
+    for (int j = 0; j < BATCH; ++j) {
+      if constexpr (VEC == 8) {
+        acc[0] += clip_four<T>(v[j].w[0], v[j].w[1]);
+        acc[1] += clip_four<T>(v[j].w[2], v[j].w[3]);
+      } else {
         float f[VEC];
         unpack(v[j], f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) { const double d = (double)f[e]; acc[(VEC == 1 ? j : e) & 3] += d * d; }
+        for (int e = 0; e < VEC; ++e) { const double d = (double)f[e]; acc[(VEC == 1 ? j : e) & 1] += d * d; }
       }
+    }
   }
 #pragma unroll 1
   for (int i = packs * VEC + threadIdx.x; i < n; i += CLIP_THREADS) { const double d = (double)to_float(in[i]); acc[0] += d * d; }
@@ -69,7 +99,7 @@ __device__ __forceinline__ void clip_squares(const T* in, int n, double (&acc)[4
 
 template <typename T, int VEC>
 __device__ __forceinline__ void clip_scale(const T* in, T* out, int n, float factor) {
-  constexpr int BATCH = VEC == 1 ? 8 : 4;
+  constexpr int BATCH = 4;
   const int packs = n / VEC;
 #pragma unroll 1
   for (int base = threadIdx.x; base < packs; base += CLIP_THREADS * BATCH) {
@@ -106,14 +136,14 @@ template <int CAP>
 __global__ void __launch_bounds__(CLIP_THREADS, 2) clip_norm_kernel(const __grid_constant__ ClipList<CAP> l, double* __restrict__ partial) {
   grid_wait();
   __shared__ double sums[CLIP_THREADS / 32];
-  double acc[4] = {0.0, 0.0, 0.0, 0.0};
+  double acc[2] = {0.0, 0.0};
   for (int c = blockIdx.x; c < l.pieces; c += gridDim.x) {
     const ClipEntry& t = l.e[clip_find(l, c)];
     const long long at = (long long)(c - t.first) * l.piece;
     const int n = (int)min((long long)l.piece, t.n - at);
     Q38_CLIP_BY_TYPE(t.type, (clip_squares<T, VEC>(reinterpret_cast<const T*>(t.in) + at, n, acc)))
   }
-  double s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+  double s = acc[0] + acc[1];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;

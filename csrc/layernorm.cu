@@ -13,6 +13,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include "f32x2.cuh"
 #include "packs.cuh"
 #include "host.h"
 #include "launch.cuh"
@@ -48,6 +49,22 @@ __device__ __forceinline__ void ln_param(const float* p, int at, float (&out)[VE
   }
 }
 
+// Pairs of neighbouring elements, for instructions that work on two at once
+template <typename T, int VEC> __device__ __forceinline__ void pairs_of(const Pack<T, VEC>& p, uint64_t (&v)[VEC / 2]) {
+  float f[VEC];
+  unpack(p, f);
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) v[i] = pair2(f[2 * i], f[2 * i + 1]);
+}
+template <int VEC> __device__ __forceinline__ void param_pairs(const float* p, int at, uint64_t (&v)[VEC / 2], float none) {
+  float f[VEC];
+  ln_param<VEC>(p, at, f, none);
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) v[i] = pair2(f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ uint64_t twice(float a) { return pair2(a, a); }
+__device__ __forceinline__ float both(uint64_t a) { const float2 f = unpair(a); return f.x + f.y; }
+
 // Sums of a and b over a group of G threads.  `scratch` belongs to the group (2 x 32 pairs, used in turn, so that one barrier per sum is enough:
 // a thread writes a half again only after a barrier that all reach after they have read it).
 template <bool WARP>
@@ -68,84 +85,161 @@ __device__ __forceinline__ float2 ln_group_sum(float a, float b, float2* scratch
   return make_float2(a, b);
 }
 
+// A thread's part of the weight and the bias: read once for all its rows where registers allow.  Read for every row they cost more of L1 than the row itself:
+// four bytes an element against two, in accesses whose lanes are 32 bytes apart (16384 x 1024 bf16: backward 30 -> 21 us).
+template <int VEC, int N, bool KEPT> struct LnParams {
+  using Unit = std::conditional_t<(VEC > 1), uint64_t, float>;
+  static constexpr int PER = VEC > 1 ? VEC / 2 : 1;
+  Unit v[KEPT ? N : 1][PER];
+  const float* p;
+  float none;
+  __device__ __forceinline__ void read(int at, Unit (&out)[PER]) const {
+    if constexpr (VEC > 1) param_pairs<VEC>(p, at, out, none); else ln_param<1>(p, at, out, none);
+  }
+  // zeros behind a row's end
+  __device__ __forceinline__ LnParams(const float* p_, float none_, int G, int t, int dim) : p(p_), none(none_) {
+    if constexpr (KEPT) {
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[c][i] = 0;
+        if ((c * G + t) * VEC < dim) read((c * G + t) * VEC, v[c]);
+      }
+    }
+  }
+  // chunk c of the thread, at element `at` of the row (inside it, unless kept)
+  __device__ __forceinline__ void get(int c, int at, Unit (&out)[PER]) const {
+    if constexpr (KEPT) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) out[i] = v[c][i];
+    } else read(at, out);
+  }
+};
+
 template <typename InT, typename OutT, int VEC, int E, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024, WARP ? (E > 16 ? 5 : 6) : 1) layer_norm_fwd_kernel(LnArgs p) {
+__global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E == 16 ? 3 : 2) layer_norm_fwd_kernel(LnArgs p) {
   grid_wait();
-  __shared__ float2 scratch[8][64];
+  __shared__ float2 scratch[WARP ? 1 : 8][64];
+  constexpr int N = E / VEC;
+  constexpr bool KEPT = WARP || E == 8;                          // otherwise 1024 threads leave no registers for it
+  constexpr bool AHEAD = E <= 16 || (VEC > 1 && sizeof(InT) == 2);
   const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
-  const long long row = (long long)blockIdx.x * p.groups + group;
-  if (row >= p.rows) return;                                     // whole groups leave; their barrier is their own
-  const InT* x = reinterpret_cast<const InT*>(p.x) + row * p.ldx;
-  OutT* y = reinterpret_cast<OutT*>(p.out) + row * p.dim;
-  int turn = 0;
-  Pack<InT, VEC> v[E / VEC];                                   // as they came: half the registers for 16-bit rows, so more of them are on their way
-  float sum = 0.f;
-#pragma unroll
-  for (int c = 0; c < E / VEC; ++c) {
-    const int at = (c * G + t) * VEC;
-    if (at < p.dim) v[c] = load_pack<InT, VEC>(x + at);
-  }
-#pragma unroll
-  for (int c = 0; c < E / VEC; ++c) {
-    if ((c * G + t) * VEC < p.dim) {
-      float f[VEC];
-      unpack(v[c], f);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sum += f[i];
-    }
-  }
   const float inv = 1.f / p.dim;
-  const float mu = ln_group_sum<WARP>(sum, 0.f, scratch[WARP ? 0 : group], turn, G, group).x * inv;
-  float ss = 0.f;
+  const long long stride = (long long)gridDim.x * p.groups;
+  const LnParams<VEC, N, KEPT> weight(p.w, 1.f, G, t, p.dim), bias(p.b, 0.f, G, t, p.dim);
+  Pack<InT, VEC> v[N] = {}, next[AHEAD ? N : 1] = {};            // rows as they came: half the registers for 16-bit types
+  auto fetch = [&](long long at_row, auto& to) {
+    if (at_row >= p.rows) return;
+    const InT* x = reinterpret_cast<const InT*>(p.x) + at_row * p.ldx;
 #pragma unroll
-  for (int c = 0; c < E / VEC; ++c) {
-    if ((c * G + t) * VEC < p.dim) {
-      float f[VEC];
-      unpack(v[c], f);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) { const float d = f[i] - mu; ss += d * d; }
+    for (int c = 0; c < N; ++c) {
+      const int at = (c * G + t) * VEC;
+      if (at < p.dim) to[c] = load_pack<InT, VEC>(x + at);
     }
-  }
-  const float r = rsqrtf(ln_group_sum<WARP>(ss, 0.f, scratch[WARP ? 0 : group], turn, G, group).x * inv + p.eps);
-  if (t == 0 && p.mean != nullptr) { p.mean[row] = mu; p.rstd[row] = r; }
+  };
+  int turn = 0;
+  long long row = (long long)blockIdx.x * p.groups + group;
+  if constexpr (AHEAD) fetch(row, next);
+#pragma unroll 1
+  for (; row < p.rows; row += stride) {
+    if constexpr (AHEAD) {
 #pragma unroll
-  for (int c = 0; c < E / VEC; ++c) {
-    const int at = (c * G + t) * VEC;
-    if (at < p.dim) {
-      float f[VEC], w[VEC], b[VEC];
-      unpack(v[c], f);
-      ln_param<VEC>(p.w, at, w, 1.f);
-      ln_param<VEC>(p.b, at, b, 0.f);
+      for (int c = 0; c < N; ++c) v[c] = next[c];
+      fetch(row + stride, next);
+    } else fetch(row, v);
+    float mu, ss = 0.f;
+    if constexpr (VEC > 1) {
+      uint64_t acc = 0;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) f[i] = (f[i] - mu) * r * w[i] + b[i];
-      store_pack<OutT, VEC>(y + at, pack<OutT, VEC>(f));
+      for (int c = 0; c < N; ++c) {
+        uint64_t f[VEC / 2];
+        pairs_of(v[c], f);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) acc = add2(acc, f[i]);
+      }
+      mu = both(acc);
+    } else {
+      mu = 0.f;
+#pragma unroll
+      for (int c = 0; c < E; ++c) { float f[1]; unpack(v[c], f); mu += f[0]; }
+    }
+    mu = ln_group_sum<WARP>(mu, 0.f, scratch[WARP ? 0 : group], turn, G, group).x * inv;
+#pragma unroll
+    for (int c = 0; c < N; ++c) forget(v[c]);
+    if constexpr (VEC > 1) {
+      const uint64_t minus = twice(-mu);
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        uint64_t f[VEC / 2], acc = 0;
+        pairs_of(v[c], f);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) { const uint64_t d = add2(f[i], minus); acc = fma2(d, d, acc); }
+        ss += (c * G + t) * VEC < p.dim ? both(acc) : 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < E; ++c) { float f[1]; unpack(v[c], f); const float d = c * G + t < p.dim ? f[0] - mu : 0.f; ss += d * d; }
+    }
+    const float r = rsqrtf(ln_group_sum<WARP>(ss, 0.f, scratch[WARP ? 0 : group], turn, G, group).x * inv + p.eps);
+    if (t == 0 && p.mean != nullptr) { p.mean[row] = mu; p.rstd[row] = r; }
+#pragma unroll
+    for (int c = 0; c < N; ++c) forget(v[c]);
+    OutT* y = reinterpret_cast<OutT*>(p.out) + row * p.dim;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      const int at = (c * G + t) * VEC;
+      if (at < p.dim) {
+        float o[VEC];
+        if constexpr (VEC > 1) {
+          uint64_t f[VEC / 2], w[VEC / 2], b[VEC / 2];
+          pairs_of(v[c], f);
+          weight.get(c, at, w);
+          bias.get(c, at, b);
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) {
+            const float2 y2 = unpair(fma2(mul2(add2(f[i], twice(-mu)), twice(r)), w[i], b[i]));
+            o[2 * i] = y2.x; o[2 * i + 1] = y2.y;
+          }
+        } else {
+          float w[1], b[1];
+          unpack(v[c], o);
+          weight.get(c, at, w);
+          bias.get(c, at, b);
+          o[0] = (o[0] - mu) * r * w[0] + b[0];
+        }
+        store_pack<OutT, VEC>(y + at, pack<OutT, VEC>(o));
+      }
     }
   }
 }
 
 // ACC: where the weight sums of a thread's columns live (registers, or shared memory for rows so long that registers would spill; each cell has one owner).
 template <typename InT, typename OutT, int VEC, int E, bool WARP, bool ACC_SMEM>
-__global__ void __launch_bounds__(ACC_SMEM ? 1024 : 512, E == 8 && VEC == 8 ? 2 : 1) layer_norm_bwd_kernel(LnArgs p) {
+__global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VEC != 8 ? 640 : 512, E == 8 && VEC == 8 ? 2 : 1) layer_norm_bwd_kernel(LnArgs p) {
   grid_wait();
-  extern __shared__ float sums[];                                // [2][dim]
+  extern __shared__ float sums[];                                // [groups][2][dim]
   __shared__ float2 scratch[16][64];
   constexpr int N = E / VEC;
   const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
   const bool wanted = p.partial != nullptr;
+  constexpr bool KEPT = !ACC_SMEM && (E != 16 || (VEC > 1 && sizeof(InT) == 2));
+  const LnParams<VEC, N, KEPT> weight(p.w, 1.f, G, t, p.dim);
   const float inv = 1.f / p.dim;
-  float aw[ACC_SMEM ? 1 : E], ab[ACC_SMEM ? 1 : E];
+  using Acc = std::conditional_t<(VEC > 1), uint64_t, float>;    // pairs of columns, or single ones
+  constexpr int ACCS = ACC_SMEM ? 1 : VEC > 1 ? E / 2 : E;
+  Acc aw[ACCS], ab[ACCS];
   if constexpr (ACC_SMEM) {
     for (int i = threadIdx.x; i < 2 * p.dim; i += blockDim.x) sums[i] = 0.f;
     __syncthreads();
   } else {
 #pragma unroll
-    for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
+    for (int i = 0; i < ACCS; ++i) aw[i] = ab[i] = 0;
   }
   const long long stride = (long long)gridDim.x * p.groups;
   long long row = (long long)blockIdx.x * p.groups + group;
   constexpr bool AHEAD = !ACC_SMEM;                              // with 1024 threads there are no registers for a row ahead
-  Pack<InT, VEC> x[N], nx[N];
-  Pack<OutT, VEC> d[N], nd[N];
+  Pack<InT, VEC> x[N], nx[N] = {};                               // zeros behind a row's end: no gradient there, so no share in any sum
+  Pack<OutT, VEC> d[N], nd[N] = {};
   float mu = 0.f, r = 0.f, nmu = 0.f, nr = 0.f;
   auto fetch = [&](long long at_row) {
     if (at_row >= p.rows) return;
@@ -171,39 +265,73 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : 512, E == 8 && VEC == 8 ? 2 
     mu = nmu; r = nr;
     if (AHEAD) fetch(row + stride);
     float s1 = 0.f, s2 = 0.f;
+    if constexpr (VEC > 1 && !ACC_SMEM) {
+      uint64_t t1 = 0, t2 = 0;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-      const int at = (c * G + t) * VEC;
-      if (at < p.dim) {
-        float xv[VEC], dv[VEC], w[VEC];
-        unpack(x[c], xv);
-        unpack(d[c], dv);
-        ln_param<VEC>(p.w, at, w, 1.f);
+      for (int c = 0; c < N; ++c) {
+        const int at = (c * G + t) * VEC;
+        uint64_t xv[VEC / 2], dv[VEC / 2], w[VEC / 2] = {};
+        pairs_of(x[c], xv);
+        pairs_of(d[c], dv);
+        if (KEPT || at < p.dim) weight.get(c, at, w);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const int e = c * VEC + i;
-          const float hat = (xv[i] - mu) * r, g = dv[i] * w[i];
-          if constexpr (ACC_SMEM) { sums[at + i] += dv[i] * hat; sums[p.dim + at + i] += dv[i]; }
-          else { aw[e] += dv[i] * hat; ab[e] += dv[i]; }
-          s1 += g; s2 += g * hat;
+        for (int i = 0; i < VEC / 2; ++i) {
+          const uint64_t hat = mul2(add2(xv[i], twice(-mu)), twice(r)), g = mul2(dv[i], w[i]);
+          aw[c * VEC / 2 + i] = fma2(dv[i], hat, aw[c * VEC / 2 + i]);
+          ab[c * VEC / 2 + i] = add2(dv[i], ab[c * VEC / 2 + i]);
+          t1 = add2(t1, g);
+          t2 = fma2(g, hat, t2);
         }
       }
-    }
-    const float2 s = ln_group_sum<WARP>(s1, s2, scratch[WARP ? 0 : group], turn, G, group);
-    if (p.out != nullptr) {
-      const float m1 = s.x * inv, m2 = s.y * inv;
-      InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
+      s1 = both(t1); s2 = both(t2);
+    } else {
 #pragma unroll
-      for (int c = 0; c < N; ++c) {                              // from the packed row again: the values themselves would take twice its registers
+      for (int c = 0; c < N; ++c) {
         const int at = (c * G + t) * VEC;
         if (at < p.dim) {
           float xv[VEC], dv[VEC], w[VEC];
           unpack(x[c], xv);
           unpack(d[c], dv);
-          ln_param<VEC>(p.w, at, w, 1.f);
+          if constexpr (VEC == 1) weight.get(c, at, w); else ln_param<VEC>(p.w, at, w, 1.f);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) xv[i] = r * (dv[i] * w[i] - m1 - (xv[i] - mu) * r * m2);
-          store_pack<InT, VEC>(dx + at, pack<InT, VEC>(xv));
+          for (int i = 0; i < VEC; ++i) {
+            const float hat = (xv[i] - mu) * r, g = dv[i] * w[i];
+            if constexpr (ACC_SMEM) { sums[at + i] += dv[i] * hat; sums[p.dim + at + i] += dv[i]; }
+            else { aw[c] += dv[i] * hat; ab[c] += dv[i]; }
+            s1 += g; s2 += g * hat;
+          }
+        }
+      }
+    }
+    const float2 s = ln_group_sum<WARP>(s1, s2, scratch[WARP ? 0 : group], turn, G, group);
+#pragma unroll
+    for (int c = 0; c < N; ++c) { forget(x[c]); forget(d[c]); }
+    if (p.out != nullptr) {
+      const float k0 = s.x * inv * r, k1 = s.y * inv * r * r;    // dx = r g - k0 - (x - mu) k1
+      InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
+#pragma unroll
+      for (int c = 0; c < N; ++c) {                              // from the packed row again: the values themselves would take twice its registers
+        const int at = (c * G + t) * VEC;
+        if (at < p.dim) {
+          float o[VEC];
+          if constexpr (VEC > 1) {
+            uint64_t xv[VEC / 2], dv[VEC / 2], w[VEC / 2];
+            pairs_of(x[c], xv);
+            pairs_of(d[c], dv);
+            weight.get(c, at, w);
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+              const float2 f = unpair(fma2(dv[i], mul2(w[i], twice(r)), fma2(add2(xv[i], twice(-mu)), twice(-k1), twice(-k0))));
+              o[2 * i] = f.x; o[2 * i + 1] = f.y;
+            }
+          } else {
+            float dv[1], w[1];
+            unpack(x[c], o);
+            unpack(d[c], dv);
+            weight.get(c, at, w);
+            o[0] = dv[0] * (w[0] * r) - ((o[0] - mu) * k1 + k0);
+          }
+          store_pack<InT, VEC>(dx + at, pack<InT, VEC>(o));
         }
       }
     }
@@ -211,22 +339,30 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : 512, E == 8 && VEC == 8 ? 2 
   if (!wanted) return;
   float* mine = p.partial + (long long)blockIdx.x * 2 * p.dim;
   if constexpr (!ACC_SMEM) {
-    for (int k = 0; k < p.groups; ++k) {                         // groups add in turn: a fixed order
-      __syncthreads();
-      if (k != group) continue;
+    // every group leaves its sums side by side, then each column is added over the groups in order
+    float* to = p.groups == 1 ? mine : sums + (long long)group * 2 * p.dim;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int at = ((e / VEC) * G + t) * VEC + e % VEC;
-        if (at < p.dim) {
-          if (p.groups == 1) { mine[at] = aw[e]; mine[p.dim + at] = ab[e]; }
-          else { sums[at] = (k ? sums[at] : 0.f) + aw[e]; sums[p.dim + at] = (k ? sums[p.dim + at] : 0.f) + ab[e]; }
-        }
+    for (int c = 0; c < N; ++c) {
+      const int at = (c * G + t) * VEC;
+      if (at < p.dim) {
+        if constexpr (VEC > 1) {
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) {
+            *reinterpret_cast<float2*>(to + at + 2 * i) = unpair(aw[c * VEC / 2 + i]);
+            *reinterpret_cast<float2*>(to + p.dim + at + 2 * i) = unpair(ab[c * VEC / 2 + i]);
+          }
+        } else { to[at] = aw[c]; to[p.dim + at] = ab[c]; }
       }
     }
     if (p.groups == 1) return;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.dim; i += blockDim.x) mine[i] = sums[i];
+  for (int i = threadIdx.x; i < 2 * p.dim; i += blockDim.x) {
+    float s = sums[i];
+    if constexpr (!ACC_SMEM)
+      for (int k = 1; k < p.groups; ++k) s += sums[(long long)k * 2 * p.dim + i];
+    mine[i] = s;
+  }
 }
 
 // Rows of any length, a CTA each, read again for every sum (the row comes from L2).  The weight sums are kept in the CTA's part of `partial`.
@@ -329,30 +465,37 @@ void by_type(at::ScalarType in, at::ScalarType out, F&& f) {
 
 template <typename InT, typename OutT, int VEC>
 void launch_fwd(LnArgs& p, cudaStream_t stream) {
-  // A warp per row up to 1024 elements: no barrier.  Eight rows per CTA.
-  auto warp_rows = [&](auto kernel) { p.groups = 8; launch(kernel, (unsigned)((p.rows + 7) / 8), 256, 0, stream, p); };
-  if (p.dim <= 256) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, 8, true>);
-  else if (p.dim <= 512) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, 16, true>);
-  else if (p.dim <= 1024) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, 32, true>);
+  // A warp per row up to 512 elements, 1024 packed ones: no barrier.  Eight rows per CTA.  (8192 x 1024 fp32 by warps 20.0 us, by groups of 128 threads 17.)
+  auto warp_rows = [&](auto kernel, int resident) {
+    p.groups = 8;
+    launch(kernel, (unsigned)std::min<long long>((p.rows + 7) / 8, resident * kNumSMs), 256, 0, stream, p);
+  };
+  if (p.dim <= 256) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, 8, true>, 4);
+  else if (p.dim <= 512) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, 16, true>, 3);
+  else if (VEC == 8 && p.dim <= 1024) warp_rows(layer_norm_fwd_kernel<InT, OutT, VEC, VEC == 8 ? 32 : 16, true>, 2);
   else {
     const bool wide = p.dim > 8192;
     const int G = group_of(p.dim, wide ? 16 : 8);
     p.groups = std::max(1, std::min(8, 256 / G));
-    const unsigned grid = (unsigned)((p.rows + p.groups - 1) / p.groups);
+    const unsigned grid = (unsigned)std::min<long long>((p.rows + p.groups - 1) / p.groups, std::max(1, 1024 / (G * p.groups)) * kNumSMs);
     if (wide) launch(layer_norm_fwd_kernel<InT, OutT, VEC, 16, false>, grid, G * p.groups, 0, stream, p);
     else launch(layer_norm_fwd_kernel<InT, OutT, VEC, 8, false>, grid, G * p.groups, 0, stream, p);
   }
 }
 
 struct BwdShape { int G, groups, ctas; };
+// Elements per thread: eight or sixteen.  The sums over a group cost some sixty instructions per thread and row, so packed rows, which have the registers, take sixteen.
+bool eight_each(int dim, bool packed16) { return dim <= 256 || (!packed16 && dim > 512 && dim <= 4096); }
+
 // Threads per row, rows per CTA and CTAs.  Eight 16-bit elements per thread take 64 registers (1024 threads per SM), eight others up to 96 (640), sixteen up to 128 (512);
 // what counts is the bytes on their way, 32 to 64 KB per SM in each case.  As many CTAs as are resident at once.
 BwdShape bwd_shape(long long rows, int dim, bool packed16) {
   if (dim > LN_LONGEST) return {1024, 1, (int)std::min<long long>(rows, kNumSMs)};
   BwdShape s;
-  const bool eight = dim <= 256 || (dim > 512 && dim <= 4096);
-  const int threads = eight && !packed16 ? 320 : 512, resident = eight ? (packed16 ? 1024 : 640) : 512;
-  s.G = dim <= 512 ? 32 : group_of(dim, dim <= 4096 ? 8 : 16);
+  const bool eight = eight_each(dim, packed16);
+  const bool warp32 = packed16 && dim > 512 && dim <= 1024;      // thirty-two per thread: a warp holds the row, no barrier
+  const int threads = warp32 ? 256 : eight && !packed16 ? 320 : 512, resident = warp32 ? 256 : eight ? (packed16 ? 1024 : 640) : 512;
+  s.G = dim <= 512 || warp32 ? 32 : group_of(dim, eight ? 8 : 16);
   s.groups = std::max(1, threads / s.G);
   s.ctas = (int)std::min<long long>((rows + s.groups - 1) / s.groups, std::max(1, resident / (s.G * s.groups)) * kNumSMs);
   return s;
@@ -361,14 +504,15 @@ BwdShape bwd_shape(long long rows, int dim, bool packed16) {
 template <typename InT, typename OutT, int VEC>
 void launch_bwd(LnArgs& p, const BwdShape& s, cudaStream_t stream) {
   p.groups = s.groups;
-  const size_t smem = (s.groups > 1 || p.dim > 8192) ? size_t(2) * p.dim * 4 : 0;
+  const size_t smem = s.groups > 1 || p.dim > 8192 ? size_t(s.groups) * 2 * p.dim * 4 : 0;        // 96 KB at most
   auto go = [&](auto kernel) {
     if (smem > 40 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     launch(kernel, (unsigned)s.ctas, s.G * s.groups, smem, stream, p);
   };
   if (p.dim <= 256) go(layer_norm_bwd_kernel<InT, OutT, VEC, 8, true, false>);
   else if (p.dim <= 512) go(layer_norm_bwd_kernel<InT, OutT, VEC, 16, true, false>);
-  else if (p.dim <= 4096) go(layer_norm_bwd_kernel<InT, OutT, VEC, 8, false, false>);
+  else if (VEC == 8 && p.dim <= 1024) go(layer_norm_bwd_kernel<InT, OutT, VEC, VEC == 8 ? 32 : 8, true, false>);
+  else if (VEC != 8 && p.dim <= 4096) go(layer_norm_bwd_kernel<InT, OutT, VEC, VEC == 8 ? 16 : 8, false, false>);
   else if (p.dim <= 8192) go(layer_norm_bwd_kernel<InT, OutT, VEC, 16, false, false>);
   else go(layer_norm_bwd_kernel<InT, OutT, VEC, 16, false, true>);
 }

@@ -51,4 +51,12 @@ template <typename T, int N> __device__ __forceinline__ Pack<T, N> pack(const fl
   return p;
 }
 
+// Hides from the compiler that `p` is what it was: without this it keeps the widened values from one use to the next, which takes the registers that packing saves.
+template <typename T, int N> __device__ __forceinline__ void forget(Pack<T, N>& p) {
+  if constexpr (N > 1) {
+#pragma unroll
+    for (int i = 0; i < int(N * sizeof(T) / 4); ++i) asm volatile("" : "+r"(p.w[i]));
+  }
+}
+
 }  // namespace q38
