@@ -6,7 +6,6 @@
 //   scale   each CTA adds up all sums in one order (a few KB from L2, instead of a third launch), takes the factor and scales its pieces
 // Bound by memory: one read for the norm, one read and one write for the scaling.  The scaling walks backwards, since what the norm read last is still in L2.
 // Where the factor is 1 and a tensor is its own result, there is nothing to write.
-#include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -15,6 +14,7 @@
 #include "packs.cuh"
 #include "host.h"
 #include "launch.cuh"
+#include "training.h"
 
 namespace q38 {
 
@@ -211,7 +211,7 @@ std::vector<ClipList<CAP>> lists_of(at::TensorList grads, at::TensorList outs, i
     if (!n) continue;
     const long long pieces = (n + piece - 1) / piece;
     if (lists.empty() || lists.back().count == CAP || lists.back().pieces + pieces > (1ll << 30)) { lists.emplace_back(); lists.back().count = lists.back().pieces = 0; lists.back().piece = piece; }
-    TORCH_CHECK(pieces < (1ll << 30), "clip_grad_norm: tensor too large");
+    TORCH_CHECK_VALUE(pieces < (1ll << 30), "clip_grad_norm: tensor too large");
     ClipList<CAP>& l = lists.back();
     ClipEntry& e = l.e[l.count++];
     e.in = grads[i].data_ptr(); e.out = outs.empty() ? const_cast<void*>(e.in) : outs[i].data_ptr(); e.n = n; e.first = l.pieces;
@@ -228,7 +228,7 @@ void run(at::TensorList grads, at::TensorList outs, int piece, double max_norm, 
   int parts = 0;
   std::vector<int> grid;
   for (const auto& l : lists) { grid.push_back(std::min(l.pieces, 2 * kNumSMs)); parts += grid.back(); }
-  const Tensor partial = at::empty({std::max(parts, 1)}, norm.options().dtype(at::kDouble));
+  const Tensor partial = new_tensor({std::max(parts, 1)}, at::kDouble, norm.device());
   double* sums = partial.data_ptr<double>();
   for (size_t i = 0, at = 0; i < lists.size(); at += grid[i++]) {
     launch(clip_norm_kernel<CAP>, grid[i], CLIP_THREADS, 0, stream, lists[i], sums + at);
@@ -252,22 +252,23 @@ struct Range { uintptr_t begin, end; size_t owner; };
 
 // The norm of all tensors together.  With `scale` the scaled tensors go to `outs`, or in place where there are none.
 Tensor clip_grad_norm(at::TensorList grads, at::TensorList outs, double max_norm, bool scale) {
-  TORCH_CHECK(!grads.empty(), "clip_grad_norm: at least one gradient required");
-  TORCH_CHECK(outs.empty() || outs.size() == grads.size(), "clip_grad_norm: as many results as gradients required");
+  TORCH_CHECK_VALUE(!grads.empty(), "clip_grad_norm: at least one gradient required");
+  TORCH_CHECK_VALUE(max_norm > 0, "clip_grad_norm: max_norm must be positive");
+  TORCH_CHECK_VALUE(outs.empty() || outs.size() == grads.size(), "clip_grad_norm: as many results as gradients required");
   const auto device = grads[0].device();
-  TORCH_CHECK(device.is_cuda(), "clip_grad_norm: CUDA tensors required");
+  TORCH_CHECK_VALUE(device.is_cuda(), "clip_grad_norm: CUDA tensors required");
   long long elements = 0;
   std::vector<Range> written, read;
   written.reserve(grads.size());
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& g = grads[i];
     const auto type = g.scalar_type();
-    TORCH_CHECK(g.device() == device, "clip_grad_norm: gradients on one device required");
-    TORCH_CHECK(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf, "clip_grad_norm: fp32, bf16 or fp16 gradients required");
-    TORCH_CHECK(g.is_non_overlapping_and_dense(), "clip_grad_norm: gradients without gaps or overlaps in memory required");
+    TORCH_CHECK_VALUE(g.device() == device, "clip_grad_norm: gradients on one device required");
+    TORCH_CHECK_VALUE(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf, "clip_grad_norm: fp32, bf16 or fp16 gradients required");
+    TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense(), "clip_grad_norm: gradients without gaps or overlaps in memory required");
     if (!outs.empty()) {
       const Tensor& o = outs[i];
-      TORCH_CHECK(o.device() == device && o.scalar_type() == type && o.sizes() == g.sizes() && (o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous())),
+      TORCH_CHECK_VALUE(o.device() == device && o.scalar_type() == type && o.sizes() == g.sizes() && (o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous())),
                   "clip_grad_norm: a result has its gradient's device, type, shape and layout");
     }
     if (!g.numel()) continue;
@@ -282,13 +283,13 @@ Tensor clip_grad_norm(at::TensorList grads, at::TensorList outs, double max_norm
   // What is written twice, or written while another tensor's values are still to be read, has no defined result
   const auto by_begin = [](const Range& a, const Range& b) { return a.begin < b.begin; };
   if (!std::is_sorted(written.begin(), written.end(), by_begin)) std::sort(written.begin(), written.end(), by_begin);
-  for (size_t i = 1; i < written.size(); ++i) TORCH_CHECK(written[i].begin >= written[i - 1].end, "clip_grad_norm: a tensor, or a part of one, is listed twice");
+  for (size_t i = 1; i < written.size(); ++i) TORCH_CHECK_VALUE(written[i].begin >= written[i - 1].end, "clip_grad_norm: a tensor, or a part of one, is listed twice");
   for (const Range& r : read) {
     auto it = std::lower_bound(written.begin(), written.end(), r, [](const Range& a, const Range& b) { return a.end <= b.begin; });
-    TORCH_CHECK(it == written.end() || it->begin >= r.end, "clip_grad_norm: a result overlaps a gradient that is not its own");
+    TORCH_CHECK_VALUE(it == written.end() || it->begin >= r.end, "clip_grad_norm: a result overlaps a gradient that is not its own");
   }
   const c10::cuda::CUDAGuard guard(device);
-  auto norm = at::empty({}, grads[0].options().dtype(at::kFloat));
+  auto norm = new_tensor({}, at::kFloat, device);
   auto stream = at::cuda::getCurrentCUDAStream();
   const int piece = piece_size(elements);
   if (grads.size() <= 64) run<64>(grads, outs, piece, max_norm, scale, norm, stream);

@@ -179,15 +179,6 @@ void cast_shadow_except(const at::Tensor& params, at::Tensor& shadow, int64_t sk
 void p2p_publish_scalar(const at::Tensor& value, std::vector<int64_t> peer_slots, int64_t rank);
 // ce.cu
 at::Tensor ce_inplace(at::Tensor& logits, const at::Tensor& target);
-// layernorm.cu
-std::vector<at::Tensor> layer_norm_fwd(const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b, double eps, at::ScalarType out_type, bool save);
-std::vector<at::Tensor> layer_norm_bwd(const at::Tensor& dy, const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b, const at::Tensor& mean,
-                                       const at::Tensor& rstd, bool want_dx, bool want_dw, bool want_db);
-// rotary.cu
-void rotary_check(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& pos, const at::Tensor& freq);
-std::pair<at::Tensor, at::Tensor> rotary_apply(const at::Tensor& q, const at::Tensor& k, const at::Tensor& pos, const at::Tensor& freq, double magnitude, bool interleaved, double sign);
-// clip.cu
-at::Tensor clip_grad_norm(at::TensorList grads, at::TensorList outs, double max_norm, bool scale);
 // conv.cu
 at::Tensor conv_silu_fwd(const at::Tensor& x, const at::Tensor& w);
 std::vector<at::Tensor> conv_silu_bwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& dy);

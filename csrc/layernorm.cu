@@ -9,14 +9,17 @@
 // In the backward a thread keeps its columns over all rows of its group, so the weight sums stay in registers; groups of a CTA are added in shared
 // memory, CTAs by a second kernel in a fixed order (no atomics: the sums have the same bits in every run).  The next row is on its way while the current
 // one is reduced.  All sums are fp32.
-#include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+
+#include <mutex>
+#include <set>
 
 #include "f32x2.cuh"
 #include "packs.cuh"
 #include "host.h"
 #include "launch.cuh"
+#include "training.h"
 
 namespace q38 {
 
@@ -440,11 +443,13 @@ __global__ void __launch_bounds__(1024) layer_norm_sums_kernel(const float* __re
 
 namespace {
 
-int param_type(const c10::optional<at::Tensor>& t) {
+int param_type(const OptTensor& t) {
   return !t.has_value() || t->scalar_type() == at::kFloat ? PARAM_F32 : t->scalar_type() == at::kBFloat16 ? PARAM_BF16 : PARAM_F16;
 }
 // Parameters as the kernels take them: fp32 (a vector in another type is converted, which costs a small launch and no branch in the kernels)
-at::Tensor param(const c10::optional<at::Tensor>& t) { return t.has_value() ? t->to(at::kFloat).contiguous() : at::Tensor(); }
+at::Tensor param(const OptTensor& t) {
+  return !t.has_value() ? at::Tensor() : t->scalar_type() == at::kFloat && t->is_contiguous() ? *t : t->to(at::kFloat).contiguous();
+}
 const float* param_ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -460,7 +465,7 @@ void by_type(at::ScalarType in, at::ScalarType out, F&& f) {
   else if (in == at::kFloat && out == at::kBFloat16) f(float{}, __nv_bfloat16{});
   else if (in == at::kBFloat16 && out == at::kBFloat16) f(__nv_bfloat16{}, __nv_bfloat16{});
   else if (in == at::kHalf && out == at::kHalf) f(__half{}, __half{});
-  else TORCH_CHECK(false, "layer_norm: output type ", out, " for an input of type ", in, " is not supported");
+  else TORCH_CHECK_VALUE(false, "layer_norm: output type ", out, " for an input of type ", in, " is not supported");
 }
 
 template <typename InT, typename OutT, int VEC>
@@ -506,7 +511,7 @@ void launch_bwd(LnArgs& p, const BwdShape& s, cudaStream_t stream) {
   p.groups = s.groups;
   const size_t smem = s.groups > 1 || p.dim > 8192 ? size_t(s.groups) * 2 * p.dim * 4 : 0;        // 96 KB at most
   auto go = [&](auto kernel) {
-    if (smem > 40 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (smem > 40 * 1024) allow_shared_memory((const void*)kernel, 128 * 1024);
     launch(kernel, (unsigned)s.ctas, s.G * s.groups, smem, stream, p);
   };
   if (p.dim <= 256) go(layer_norm_bwd_kernel<InT, OutT, VEC, 8, true, false>);
@@ -517,35 +522,69 @@ void launch_bwd(LnArgs& p, const BwdShape& s, cudaStream_t stream) {
   else go(layer_norm_bwd_kernel<InT, OutT, VEC, 16, false, true>);
 }
 
-void check_params(const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b) {
+void check_params(const at::Tensor& x, const OptTensor& w, const OptTensor& b) {
   for (const auto* t : {&w, &b})
     if (t->has_value())
-      TORCH_CHECK((*t)->device() == x.device() && (*t)->dim() == 1 && (*t)->size(0) == x.size(1) &&
-                  ((*t)->scalar_type() == at::kFloat || (*t)->scalar_type() == at::kBFloat16 || (*t)->scalar_type() == at::kHalf),
-                  "layer_norm: weight and bias are fp32, bf16 or fp16 vectors of the last dimension's length on the input's device");
+      TORCH_CHECK_VALUE((*t)->device() == x.device() && (*t)->dim() == 1 && (*t)->size(0) == x.size(-1) &&
+                        ((*t)->scalar_type() == at::kFloat || (*t)->scalar_type() == at::kBFloat16 || (*t)->scalar_type() == at::kHalf),
+                        "layer_norm: weight and bias are fp32, bf16 or fp16 vectors of the last dimension's length on the input's device");
 }
+
+// A tensor as rows with contiguous columns and one distance between them; copied where it has not that already.
+struct Rows {
+  at::Tensor held;
+  long long rows, ld;
+  explicit Rows(const at::Tensor& t) : held(t), rows(1), ld(t.size(-1)) {
+    const auto sizes = t.sizes(), strides = t.strides();
+    const int64_t last = t.dim() - 1;
+    bool ok = strides[last] == 1 || sizes[last] == 1, set = false;
+    long long next = 0;
+    for (int64_t i = last - 1; i >= 0; --i) {
+      rows *= sizes[i];
+      if (sizes[i] == 1) continue;
+      if (!set) { ld = strides[i]; set = true; }
+      else if (strides[i] != next) ok = false;
+      next = strides[i] * sizes[i];
+    }
+    if (!ok && rows) { held = t.contiguous(); ld = t.size(-1); }
+  }
+};
 
 }  // namespace
 
-// x [rows, dim] with contiguous columns -> {y, mean, rstd}; without `save` the last two are empty.
-std::vector<at::Tensor> layer_norm_fwd(const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b, double eps, at::ScalarType out_type, bool save) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) > 0 && (x.stride(1) == 1 || x.size(1) == 1) && x.size(1) <= INT_MAX / 2, "layer_norm: [rows, dim] CUDA input with contiguous columns required");
+void allow_shared_memory(const void* kernel, int bytes) {
+  static std::mutex mutex;
+  static std::set<std::pair<const void*, int>> done;
+  int device = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&device));
+  const std::lock_guard<std::mutex> lock(mutex);
+  if (done.count({kernel, device})) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.insert({kernel, device});
+}
+
+std::pair<at::Tensor, at::Tensor> layer_norm_fwd(const at::Tensor& x, const OptTensor& w, const OptTensor& b, double eps, at::ScalarType out_type, bool save) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() > 0 && x.size(-1) > 0 && x.size(-1) <= INT_MAX / 2, "layer_norm: a CUDA input with a last dimension that is not empty is required");
+  TORCH_CHECK_VALUE(eps >= 0, "layer_norm: eps must not be negative");
   check_params(x, w, b);
   const c10::cuda::CUDAGuard guard(x.device());
+  const Rows in(x);
   LnArgs p{};
-  p.rows = x.size(0); p.dim = (int)x.size(1); p.ldx = x.stride(0); p.eps = (float)eps;
-  auto y = at::empty({p.rows, p.dim}, x.options().dtype(out_type));
-  auto stats = at::empty({save ? 2 : 0, p.rows}, x.options().dtype(at::kFloat));
-  auto mean = save ? stats[0] : stats, rstd = save ? stats[1] : stats;
+  p.rows = in.rows; p.dim = (int)x.size(-1); p.ldx = in.ld; p.eps = (float)eps;
+  auto y = new_tensor(x.sizes(), out_type, x.device());
   const at::Tensor wf = param(w), bf = param(b);
-  p.x = x.data_ptr(); p.out = y.data_ptr(); p.w = param_ptr(wf); p.b = param_ptr(bf);
-  if (save) { p.mean = mean.data_ptr<float>(); p.rstd = rstd.data_ptr<float>(); }
-  by_type(x.scalar_type(), out_type, [&](auto in, auto out) {
-    using InT = decltype(in);
-    using OutT = decltype(out);
+  p.x = in.held.data_ptr(); p.out = y.data_ptr(); p.w = param_ptr(wf); p.b = param_ptr(bf);
+  at::Tensor stats;
+  if (save) {
+    stats = new_tensor({2, p.rows}, at::kFloat, x.device());
+    p.mean = stats.data_ptr<float>(); p.rstd = p.mean + p.rows;
+  }
+  by_type(x.scalar_type(), out_type, [&](auto in_zero, auto out_zero) {
+    using InT = decltype(in_zero);
+    using OutT = decltype(out_zero);
     constexpr int VEC = 16 / sizeof(InT);
     if (p.rows == 0) return;
-    TORCH_CHECK(p.rows < (1ll << 31), "layer_norm: at most 2^31 - 1 rows");
+    TORCH_CHECK_VALUE(p.rows < (1ll << 31), "layer_norm: at most 2^31 - 1 rows");
     auto stream = at::cuda::getCurrentCUDAStream();
     const bool vec = p.dim % VEC == 0 && p.ldx % VEC == 0 && on16(p.x) && on16(p.out) && on16(p.w) && on16(p.b);
     if (p.dim > LN_LONGEST) launch(layer_norm_long_kernel<InT, OutT>, (unsigned)std::min<long long>(p.rows, 2 * kNumSMs), 1024, 0, stream, p, false);
@@ -554,38 +593,43 @@ std::vector<at::Tensor> layer_norm_fwd(const at::Tensor& x, const c10::optional<
     C10_CUDA_KERNEL_LAUNCH_CHECK();
     count_launch();
   });
-  return {y, mean, rstd};
+  return {y, stats};
 }
 
-// {dx, dw, db}: empty where not wanted.
-std::vector<at::Tensor> layer_norm_bwd(const at::Tensor& dy, const at::Tensor& x, const c10::optional<at::Tensor>& w, const c10::optional<at::Tensor>& b, const at::Tensor& mean,
-                                       const at::Tensor& rstd, bool want_dx, bool want_dw, bool want_db) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1) && dy.device() == x.device() && dy.sizes() == x.sizes() && (dy.stride(1) == 1 || dy.size(1) == 1) &&
-              mean.numel() == x.size(0) && rstd.numel() == x.size(0), "layer_norm_bwd: bad inputs");
-  check_params(x, w, b);
-  const c10::cuda::CUDAGuard guard(x.device());
+std::array<at::Tensor, 3> layer_norm_bwd(const at::Tensor& dy_, const at::Tensor& x_, const OptTensor& w, const OptTensor& b, const at::Tensor& stats, bool want_dx, bool want_dw, bool want_db) {
+  TORCH_CHECK(x_.is_cuda() && dy_.device() == x_.device() && dy_.sizes() == x_.sizes(), "layer_norm: a gradient of the result's shape and device required");
+  check_params(x_, w, b);
+  const c10::cuda::CUDAGuard guard(x_.device());
+  const Rows x(x_), dy(dy_);
+  const auto device = x_.device();
   LnArgs p{};
-  p.rows = x.size(0); p.dim = (int)x.size(1); p.ldx = x.stride(0); p.lddy = dy.stride(0);
-  auto dx = want_dx ? at::empty({p.rows, p.dim}, x.options()) : at::Tensor();
-  auto dw = want_dw ? at::empty_like(*w) : at::Tensor(), db = want_db ? at::empty_like(*b) : at::Tensor();
+  p.rows = x.rows; p.dim = (int)x_.size(-1); p.ldx = x.ld; p.lddy = dy.ld;
+  at::Tensor dx, dw, db;
+  if (want_dx) dx = new_tensor(x_.sizes(), x_.scalar_type(), device);
+  if (want_dw) dw = new_tensor({p.dim}, w->scalar_type(), device);
+  if (want_db) db = new_tensor({p.dim}, b->scalar_type(), device);
   if (p.rows == 0) {
     if (want_dw) dw.zero_();
     if (want_db) db.zero_();
     return {dx, dw, db};
   }
-  const int per16 = 16 / (int)x.element_size();
+  TORCH_CHECK(stats.numel() == 2 * p.rows, "layer_norm: statistics of every row required");
+  const int per16 = 16 / (int)x_.element_size();
   const at::Tensor wf = param(w);
-  p.x = x.data_ptr(); p.dy = dy.data_ptr(); p.w = param_ptr(wf);
+  p.x = x.held.data_ptr(); p.dy = dy.held.data_ptr(); p.w = param_ptr(wf);
   p.out = want_dx ? dx.data_ptr() : nullptr;
+  p.mean = stats.data_ptr<float>(); p.rstd = p.mean + p.rows;
   const bool vec = p.dim % per16 == 0 && p.ldx % per16 == 0 && p.lddy % per16 == 0 && on16(p.x) && on16(p.dy) && on16(p.out) && on16(p.w);
   const BwdShape s = bwd_shape(p.rows, p.dim, vec && per16 == 8);
   at::Tensor partial;
-  if (want_dw || want_db) partial = at::empty({s.ctas, 2, p.dim}, x.options().dtype(at::kFloat));
-  p.mean = mean.data_ptr<float>(); p.rstd = rstd.data_ptr<float>(); p.partial = partial.defined() ? partial.data_ptr<float>() : nullptr;
+  if (want_dw || want_db) {
+    partial = new_tensor({s.ctas, 2, p.dim}, at::kFloat, device);
+    p.partial = partial.data_ptr<float>();
+  }
   auto stream = at::cuda::getCurrentCUDAStream();
-  by_type(x.scalar_type(), dy.scalar_type(), [&](auto in, auto out) {
-    using InT = decltype(in);
-    using OutT = decltype(out);
+  by_type(x_.scalar_type(), dy_.scalar_type(), [&](auto in_zero, auto out_zero) {
+    using InT = decltype(in_zero);
+    using OutT = decltype(out_zero);
     constexpr int VEC = 16 / sizeof(InT);
     if (p.dim > LN_LONGEST) launch(layer_norm_long_kernel<InT, OutT>, (unsigned)s.ctas, 1024, 0, stream, p, true);
     else if (vec) launch_bwd<InT, OutT, VEC>(p, s, stream);

@@ -9,13 +9,13 @@
 // Bound by memory: every element is read and written once.  A CTA takes a few tokens, makes their cosines and sines once for all heads (shared memory), and
 // walks the tokens' heads in pieces of 16 bytes: a piece of each half, two neighbouring pieces of an interleaved head, or two that pass through.
 // Tensors are addressed by their strides, so packed projections and head-major tensors are read in place.
-#include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "packs.cuh"
 #include "host.h"
 #include "launch.cuh"
+#include "training.h"
 
 namespace q38 {
 
@@ -135,6 +135,7 @@ namespace {
 
 using at::Tensor;
 
+Tensor like(const Tensor& t) { return t.is_contiguous() ? new_tensor(t.sizes(), t.scalar_type(), t.device()) : at::empty_like(t); }
 Tensor with_columns(const Tensor& t) { return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous(); }
 
 RotarySide side_of(const Tensor& in, const Tensor& out) {
@@ -160,10 +161,9 @@ void launch_rotary(RotaryArgs& p, bool interleaved, cudaStream_t stream) {
   if (half) n = std::max<long long>(1, std::min<long long>(n, 4096 / half));
   p.per_cta = (int)n;
   const long long grid = (p.tokens + n - 1) / n;
-  TORCH_CHECK(grid < (1ll << 31) && per_token * n < (1ll << 30), "rotary: tensor too large");
+  TORCH_CHECK_VALUE(grid < (1ll << 31) && per_token * n < (1ll << 30), "rotary: tensor too large");
   const size_t smem = size_t(p.per_cta) * half * sizeof(float2);
   auto go = [&](auto kernel) {
-    if (smem > 48 * 1024) C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     launch(kernel, (unsigned)grid, ROT_THREADS, smem, stream, p);
   };
   if (interleaved) go(rotary_kernel<T, VEC, true>); else go(rotary_kernel<T, VEC, false>);
@@ -190,8 +190,8 @@ std::pair<Tensor, Tensor> rotary_apply(const Tensor& q_in, const Tensor& k_in, c
   const Tensor& any = q_in.defined() ? q_in : k_in;
   const c10::cuda::CUDAGuard guard(any.device());
   Tensor q, k, qo, ko;
-  if (q_in.defined()) { q = with_columns(q_in); qo = at::empty_like(q); }
-  if (k_in.defined()) { k = with_columns(k_in); ko = at::empty_like(k); }
+  if (q_in.defined()) { q = with_columns(q_in); qo = like(q); }
+  if (k_in.defined()) { k = with_columns(k_in); ko = like(k); }
   RotaryArgs p{};
   int fit = 8;
   if (q.defined()) { p.q = side_of(q, qo); fit = std::min({fit, packs_fit(q), packs_fit(qo)}); }
@@ -211,17 +211,17 @@ std::pair<Tensor, Tensor> rotary_apply(const Tensor& q_in, const Tensor& k_in, c
   return {qo, ko};
 }
 
-void rotary_check(const Tensor& q, const c10::optional<Tensor>& k, const Tensor& pos, const Tensor& freq) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 4 && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf || q.scalar_type() == at::kFloat),
+void rotary_check(const Tensor& q, const OptTensor& k, const Tensor& pos, const Tensor& freq) {
+  TORCH_CHECK_VALUE(q.is_cuda() && q.dim() == 4 && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf || q.scalar_type() == at::kFloat),
               "rotary: bf16, fp16 or fp32 CUDA tensors [batch, seq, heads, dim] required");
-  TORCH_CHECK(!k.has_value() || (k->device() == q.device() && k->scalar_type() == q.scalar_type() && k->dim() == 4 && k->size(0) == q.size(0) && k->size(1) == q.size(1) && k->size(3) == q.size(3)),
+  TORCH_CHECK_VALUE(!k.has_value() || (k->device() == q.device() && k->scalar_type() == q.scalar_type() && k->dim() == 4 && k->size(0) == q.size(0) && k->size(1) == q.size(1) && k->size(3) == q.size(3)),
               "rotary: keys have the type, device, batch, length and head size of the queries");
-  TORCH_CHECK(pos.device() == q.device() && (pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) &&
+  TORCH_CHECK_VALUE(pos.device() == q.device() && (pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt) &&
               ((pos.dim() == 1 && pos.size(0) == q.size(1)) || (pos.dim() == 2 && pos.size(1) == q.size(1) && (pos.size(0) == q.size(0) || pos.size(0) == 1))),
               "rotary: whole positions [seq], [1, seq] or [batch, seq] on the queries' device required");
-  TORCH_CHECK(freq.device() == q.device() && freq.scalar_type() == at::kDouble && freq.dim() == 1 && freq.is_contiguous() && 2 * freq.size(0) <= q.size(3),
-              "rotary: contiguous 64-bit frequencies on the queries' device, at most half a head of them, required");
-  TORCH_CHECK(q.size(1) < (1ll << 31) && q.size(3) <= 8192, "rotary: sequence or head too long");
+  TORCH_CHECK_VALUE(freq.device() == q.device() && freq.scalar_type() == at::kDouble && freq.dim() == 1 && 2 * freq.size(0) <= q.size(3),
+              "rotary: 64-bit frequencies on the queries' device, at most half a head of them, required");
+  TORCH_CHECK_VALUE(q.size(1) < (1ll << 31) && q.size(3) <= 8192, "rotary: sequence or head too long");
 }
 
 }  // namespace q38

@@ -1,86 +1,173 @@
-// Autograd nodes of the operators around a training step's products (layer norm, rotary positions) and the registration of these and of the
-// gradient norm.  The nodes are C++: a node written in Python costs 10 to 20 us per pass, more than the kernels of a short sequence.
+// Autograd nodes of the operators around a training step's products, and their registration.  The nodes are written out in C++: one in Python costs 10 to 20 us
+// per pass, torch's own wrapper for C++ functions half of that, and the kernels of a short sequence take 2 to 5.
 #include <ATen/ATen.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
-#include "host.h"
+#include "training.h"
 
 namespace q38 {
-// vocab_loss.cu
-std::vector<at::Tensor> vocab_loss_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, int64_t reduction, const at::Tensor& err);
-std::vector<at::Tensor> vocab_loss_bwd(const at::Tensor& g, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& lse2, const at::Tensor& count,
-                                       int64_t reduction, bool want_dh, bool fp32_dh, bool want_dw, bool fp32_dw, const c10::optional<at::Tensor>& grad, int64_t workspace,
-                                       const at::Tensor& err);
-
 namespace {
 
 using at::Tensor;
-using OptTensor = c10::optional<Tensor>;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
-bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+void first_order_only(const char* name) { TORCH_CHECK(!at::GradMode::is_enabled(), name, ": a gradient of the gradient is not available"); }
 
 // ---- layer norm ---------------------------------------------------------------------------------------------------------------
-// [rows, dim] with contiguous columns and one distance between rows, without a copy where x has that already
-Tensor as_rows(const Tensor& x) {
-  const auto r = x.reshape({-1, x.size(-1)});
-  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
-}
-
-struct LayerNorm : public torch::autograd::Function<LayerNorm> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, at::ScalarType out_type) {
-    auto out = layer_norm_fwd(as_rows(x), w, b, eps, out_type, true);
-    ctx->save_for_backward({x, w.value_or(Tensor()), b.value_or(Tensor()), out[1], out[2]});
-    return out[0].view(x.sizes());
+struct LayerNormBackward : public Node {
+  SavedVariable x, w;
+  Tensor stats;
+  OptTensor b;                     // of the bias only its type and length count: a detached alias, so that changing it is allowed
+  std::string name() const override { return "Q38LayerNormBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data(); w.reset_data(); stats.reset();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm: a gradient of the gradient is not available");
-    auto saved = ctx->get_saved_variables();
-    const OptTensor w = optional_of(saved[1]), b = optional_of(saved[2]);
-    const size_t b_edge = w.has_value() ? 2 : 1;                   // edges are counted over the tensors that were given
-    auto out = layer_norm_bwd(as_rows(grads[0]), as_rows(saved[0]), w, b, saved[3], saved[4], ctx->needs_input_grad(0), w.has_value() && ctx->needs_input_grad(1),
-                              b.has_value() && ctx->needs_input_grad(b_edge));
-    return {out[0].defined() ? out[0].view(saved[0].sizes()) : out[0], out[1], out[2], Tensor(), Tensor()};
+  variable_list apply(variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    first_order_only("layer_norm");
+    if (!grads[0].defined()) return variable_list(3);
+    auto self = shared_from_this();
+    const Tensor xs = x.unpack(self), ws = w.unpack(self);
+    auto out = layer_norm_bwd(grads[0], xs, optional_of(ws), b, stats, task_should_compute_output(0), ws.defined() && task_should_compute_output(1),
+                              b.has_value() && task_should_compute_output(2));
+    return {out[0], out[1], out[2]};
   }
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, c10::optional<at::ScalarType> out_type) {
-  TORCH_CHECK(x.dim() > 0 && x.size(-1) > 0, "layer_norm: an input with a last dimension that is not empty required");
-  const at::ScalarType to = out_type.value_or(x.scalar_type());
-  if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(w) || wants_grad(b))) return LayerNorm::apply(x, w, b, eps, to);
-  return layer_norm_fwd(as_rows(x), w, b, eps, to, false)[0].view(x.sizes());
+  const Tensor wt = w.value_or(Tensor()), bt = b.value_or(Tensor());
+  const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(wt) || wants_grad(bt));
+  Tensor y, stats;
+  {
+    const at::NoGradGuard none;
+    std::tie(y, stats) = layer_norm_fwd(x, w, b, eps, out_type.value_or(x.scalar_type()), grad);
+  }
+  if (grad) {
+    auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, wt, bt));
+    node->x = SavedVariable(x, false);
+    node->w = SavedVariable(wt, false);
+    node->stats = stats;
+    if (b.has_value()) node->b = b->detach();
+    torch::autograd::set_history(y, node);
+  }
+  return y;
 }
 
 // ---- rotary positions ------------------------------------------------------------------------------------------------------------
-struct Rotary : public torch::autograd::Function<Rotary> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const Tensor& pos, const Tensor& freq, double magnitude, bool interleaved) {
-    auto [qo, ko] = rotary_apply(q, k.value_or(Tensor()), pos, freq, magnitude, interleaved, 1.0);
-    ctx->save_for_backward({pos, freq});
-    ctx->saved_data["magnitude"] = magnitude;
-    ctx->saved_data["interleaved"] = interleaved;
-    ctx->set_materialize_grads(false);
-    return k.has_value() ? variable_list{qo, ko} : variable_list{qo};
+struct RotaryBackward : public Node {
+  SavedVariable pos, freq;
+  double magnitude;
+  bool interleaved;
+  std::string name() const override { return "Q38RotaryBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    pos.reset_data(); freq.reset_data();
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), "rotary: a gradient of the gradient is not available");
-    auto saved = ctx->get_saved_variables();
-    const bool keys = grads.size() > 1;
-    const Tensor dq = grads[0].defined() && ctx->needs_input_grad(0) ? grads[0] : Tensor();
-    const Tensor dk = keys && grads[1].defined() && ctx->needs_input_grad(1) ? grads[1] : Tensor();
-    std::pair<Tensor, Tensor> out;
-    if (dq.defined() || dk.defined()) out = rotary_apply(dq, dk, saved[0], saved[1], ctx->saved_data["magnitude"].toDouble(), ctx->saved_data["interleaved"].toBool(), -1.0);
-    return {out.first, out.second, Tensor(), Tensor(), Tensor(), Tensor()};
+  variable_list apply(variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    first_order_only("rotary");
+    const Tensor dq = task_should_compute_output(0) ? grads[0] : Tensor(), dk = grads.size() > 1 && task_should_compute_output(1) ? grads[1] : Tensor();
+    if (!dq.defined() && !dk.defined()) return variable_list(2);
+    auto out = rotary_apply(dq, dk, pos.unpack(), freq.unpack(), magnitude, interleaved, -1.0);
+    return {out.first, out.second};
   }
 };
 
-std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& pos, const Tensor& freq, double magnitude, bool interleaved) {
+std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& pos, const Tensor& frequencies, double magnitude, bool interleaved) {
+  const Tensor freq = frequencies.is_contiguous() ? frequencies : frequencies.contiguous();
   rotary_check(q, k, pos, freq);
-  if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k))) return Rotary::apply(q, k, pos, freq, magnitude, interleaved);
-  auto [qo, ko] = rotary_apply(q, k.value_or(Tensor()), pos, freq, magnitude, interleaved, 1.0);
-  return k.has_value() ? std::vector<Tensor>{qo, ko} : std::vector<Tensor>{qo};
+  const Tensor kt = k.value_or(Tensor());
+  const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(kt));
+  std::pair<Tensor, Tensor> out;
+  {
+    const at::NoGradGuard none;                                    // layouts that need a copy
+    out = rotary_apply(q, kt, pos, freq, magnitude, interleaved, 1.0);
+  }
+  if (grad) {
+    auto node = std::shared_ptr<RotaryBackward>(new RotaryBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(q, kt));
+    node->pos = SavedVariable(pos, false);
+    node->freq = SavedVariable(freq, false);
+    node->magnitude = magnitude;
+    node->interleaved = interleaved;
+    torch::autograd::set_history(out.first, node);
+    if (k.has_value()) torch::autograd::set_history(out.second, node);
+  }
+  return k.has_value() ? std::vector<Tensor>{out.first, out.second} : std::vector<Tensor>{out.first};
+}
+
+// ---- vocabulary loss ---------------------------------------------------------------------------------------------------------------
+struct VocabLossBackward : public Node {
+  SavedVariable hidden, weight, target;      // hidden and weight in bf16, as the products take them
+  Tensor lse2, count, err, parameter;        // parameter: of the trainer's arena, its gradient buffer is added to
+  std::vector<int64_t> shape;                // of the hidden states as they were given
+  int64_t reduction, workspace;
+  bool fp32_dh, fp32_dw;
+  std::string name() const override { return "Q38VocabLossBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    hidden.reset_data(); weight.reset_data(); target.reset_data();
+    lse2.reset(); count.reset(); parameter.reset();
+  }
+  variable_list apply(variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    first_order_only("vocabulary_cross_entropy");
+    if (!grads[0].defined()) return variable_list(2);
+    const Tensor h = hidden.unpack(), w = weight.unpack(), t = target.unpack(), g = grads[0].reshape({-1}).to(at::kFloat).contiguous();
+    const bool want_dw = task_should_compute_output(1);
+    Tensor buffer;
+    if (want_dw && parameter.defined()) {
+      const Tensor& own = parameter.grad();
+      if (own.defined() && own.scalar_type() == at::kFloat && own.is_contiguous() && own.size(1) % 4 == 0 && (reinterpret_cast<uintptr_t>(own.data_ptr()) & 15) == 0) buffer = own;
+    }
+    auto out = vocab_loss_bwd(g, h.view({-1, w.size(1)}), w, t.view({-1}), lse2, count, reduction, task_should_compute_output(0), fp32_dh, want_dw, fp32_dw, buffer, workspace, err);
+    return {out.first.defined() ? out.first.view(shape) : out.first, out.second};
+  }
+};
+
+// hidden [..., h]; weight [vocabulary, h] and the same in bf16; target of hidden's leading shape.
+Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weight16, const Tensor& target, int64_t reduction, bool managed, int64_t workspace, const Tensor& err) {
+  TORCH_CHECK_VALUE(weight.dim() == 2 && hidden.dim() >= 1 && hidden.size(-1) == weight.size(1) && weight.numel() > 0,
+                    "vocabulary_cross_entropy: hidden [..., h] and weight [vocabulary, h] required");
+  TORCH_CHECK_VALUE(target.sizes() == hidden.sizes().slice(0, hidden.dim() - 1) && target.scalar_type() == at::kLong, "vocabulary_cross_entropy: int64 targets of hidden's leading shape required");
+  for (const Tensor* t : {&hidden, &weight})
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat, "vocabulary_cross_entropy: bf16 or fp32 hidden states and weight required");
+  TORCH_CHECK_VALUE(hidden.is_cuda() && weight.device() == hidden.device() && target.device() == hidden.device(), "vocabulary_cross_entropy: hidden, weight and target on one device required");
+  const bool grad = at::GradMode::is_enabled() && (wants_grad(hidden) || wants_grad(weight));
+  Tensor h16, t, loss, lse2, count;
+  {
+    const at::NoGradGuard none;
+    // kept as they were given where nothing has to be converted or copied: a change before the backward is then noticed
+    h16 = hidden.scalar_type() == at::kBFloat16 ? hidden : hidden.to(at::kBFloat16);
+    t = target.is_contiguous() ? target : target.contiguous();
+    const Tensor h2 = h16.dim() == 2 ? h16 : h16.reshape({-1, h16.size(-1)});
+    if (h16.dim() != 2 && !h16.is_contiguous()) h16 = h2;
+    auto out = vocab_loss_fwd(h2, weight16, t.dim() == 1 ? t : t.view({-1}), target.sizes(), reduction, err);
+    loss = out[0]; lse2 = out[1]; count = out[2];
+  }
+  if (grad) {
+    auto node = std::shared_ptr<VocabLossBackward>(new VocabLossBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(hidden, weight));
+    node->hidden = SavedVariable(h16, false);
+    node->weight = SavedVariable(weight16, false);
+    node->target = SavedVariable(t, false);
+    node->lse2 = lse2; node->count = count; node->err = err;
+    if (managed) node->parameter = weight;
+    node->shape = hidden.sizes().vec();
+    node->reduction = reduction; node->workspace = workspace;
+    node->fp32_dh = hidden.scalar_type() == at::kFloat; node->fp32_dw = weight.scalar_type() == at::kFloat;
+    torch::autograd::set_history(loss, node);
+  }
+  return loss;
 }
 
 }  // namespace
@@ -89,9 +176,7 @@ std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& po
 TORCH_LIBRARY_FRAGMENT(q38, m) {
   m.def("layer_norm(Tensor x, Tensor? w, Tensor? b, float eps, ScalarType? out_dtype=None) -> Tensor", &q38::layer_norm);
   m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor frequencies, float magnitude, bool interleaved) -> Tensor[]", &q38::rotary);
-  m.def("vocab_loss_fwd(Tensor hidden, Tensor weight, Tensor target, int reduction, Tensor(a!) err) -> Tensor[]", &q38::vocab_loss_fwd);
-  m.def("vocab_loss_bwd(Tensor g, Tensor hidden, Tensor weight, Tensor target, Tensor lse2, Tensor count, int reduction, bool want_dh, bool fp32_dh, bool want_dw, bool fp32_dw, "
-        "Tensor(b!)? grad, int workspace, Tensor(a!) err) -> Tensor[]", &q38::vocab_loss_bwd);
+  m.def("vocab_loss(Tensor hidden, Tensor weight, Tensor weight16, Tensor target, int reduction, bool managed, int workspace, Tensor(a!) err) -> Tensor", &q38::vocab_loss);
   m.def("grad_norm(Tensor[] grads) -> Tensor", [](at::TensorList g) { return q38::clip_grad_norm(g, {}, 1.0, false); });
   m.def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm) -> Tensor", [](at::TensorList g, double m) { return q38::clip_grad_norm(g, {}, m, true); });
   m.def("clip_grad_norm_out(Tensor[] grads, Tensor(a!)[] out, float max_norm) -> Tensor", [](at::TensorList g, at::TensorList o, double m) { return q38::clip_grad_norm(g, o, m, true); });

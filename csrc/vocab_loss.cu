@@ -12,7 +12,6 @@
 // The kernel follows csrc/gemm_persistent.cu: one CTA per SM, warp 0 loads by TMA, one lane of warp 1 issues the MMAs into one of two accumulators, and eight
 // warps (two warpgroups on alternate 32-column chunks) read the other.  Tiles are walked with the rows fastest, in groups of rows whose hidden states
 // stay in L2: all SMs work on the same few columns of W, which so comes from memory once per group.
-#include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -20,6 +19,7 @@
 #include "ptx.cuh"
 #include "host.h"
 #include "launch.cuh"
+#include "training.h"
 
 namespace q38 {
 
@@ -271,8 +271,8 @@ __global__ void __launch_bounds__(1024) vocab_join_kernel(const float2* __restri
   loss[mine] = inside ? (float)(l2 * 0.69314718055994530942 - (double)target_logit[mine]) : 0.f;
 }
 
-// Sum of all losses and number of rows that count, by one CTA in a fixed order: out[0] the sum or the mean over those rows, out[1] that number (at least 1).
-__global__ void __launch_bounds__(1024) vocab_sum_kernel(const float* __restrict__ loss, const long long* __restrict__ target, int rows, int vocab, bool mean, float* out) {
+// Sum of all losses and number of rows that count, by one CTA in a fixed order: `total` the sum or the mean over those rows, `number` how many they are (at least 1).
+__global__ void __launch_bounds__(1024) vocab_sum_kernel(const float* __restrict__ loss, const long long* __restrict__ target, int rows, int vocab, bool mean, float* total, float* number) {
   grid_wait();
   __shared__ double sums[32];
   __shared__ int counts[32];
@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(1024) vocab_sum_kernel(const float* __restrict
   if (threadIdx.x != 0) return;
   for (int w = 1; w < 32; ++w) { s += sums[w]; n += counts[w]; }
   n = max(n, 1);
-  out[0] = (float)(mean ? s / n : s);
-  out[1] = (float)n;
+  *total = (float)(mean ? s / n : s);
+  *number = (float)n;
 }
 
 // out [rows, cols] = sum of `slabs` fp32 matrices (rows of ldp elements, a multiple of 4), in order, as bf16 or fp32: a warp per row, four columns per lane
@@ -365,7 +365,7 @@ int64_t padded(int64_t n) { return (n + 63) / 64 * 64; }
 Tensor tma_rows(const Tensor& t, cudaStream_t stream) {
   const int64_t n = t.size(1);
   if ((t.stride(1) == 1 || n == 1) && (t.stride(0) >= n || t.size(0) == 1) && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) return t;
-  auto view = at::empty({t.size(0), padded(n)}, t.options()).narrow(1, 0, n);
+  auto view = new_tensor({t.size(0), padded(n)}, t.scalar_type(), t.device()).narrow(1, 0, n);
   copy_rows(t, view, stream);
   return view;
 }
@@ -410,7 +410,7 @@ void launch_tiles(const Tensor& h, const Tensor& w, int64_t first_col, int64_t c
   const CUtensorMap ta = make_tmap_box(h.data_ptr(), 2, p.K, p.rows, 1, h.stride(0), 0, V_BM, 128);
   const CUtensorMap tb = make_tmap_box(reinterpret_cast<const __nv_bfloat16*>(w.data_ptr()) + first_col * w.stride(0), 2, p.K, cols, 1, w.stride(0), 0, p.bn, 128);
   auto kernel = vocab_tiles_kernel<GRAD>;
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+  allow_shared_memory((const void*)kernel, 227 * 1024);
   launch(kernel, (unsigned)std::min(p.items, kNumSMs), V_THREADS, smem, stream, ta, tb, out ? *out : ta, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   count_launch();
@@ -428,21 +428,18 @@ void check(const Tensor& h, const Tensor& w, const Tensor& target) {
 
 }  // namespace
 
-// reduction: 0 none, 1 sum, 2 mean over the rows that count.  Returns {loss ([rows] or 0-dim), lse2 [rows], count (one element; empty without a reduction)}.
-std::vector<Tensor> vocab_loss_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& target, int64_t reduction, const Tensor& err) {
+std::array<Tensor, 3> vocab_loss_fwd(const Tensor& hidden, const Tensor& weight, const Tensor& target, at::IntArrayRef shape, int64_t reduction, const Tensor& err) {
   check(hidden, weight, target);
-  const c10::cuda::CUDAGuard guard(hidden.device());
-  const auto f32 = hidden.options().dtype(at::kFloat);
+  const auto device = hidden.device();
+  const c10::cuda::CUDAGuard guard(device);
   const int64_t rows = hidden.size(0), vocab = weight.size(0);
-  auto loss = at::empty({rows}, f32), lse2 = at::empty({rows}, f32);
-  auto out = at::empty({reduction ? 2 : 0}, f32);
+  auto loss = new_tensor(reduction ? at::IntArrayRef(rows) : shape, at::kFloat, device), lse2 = new_tensor({rows}, at::kFloat, device);
   auto stream = at::cuda::getCurrentCUDAStream();
   if (rows) {
     const Tensor h = tma_rows(hidden, stream), w = tma_rows(weight, stream);
     VocabArgs p{};
     const int bn = tile_width(rows, vocab);
-    auto partial = at::empty({2 * ((vocab + bn - 1) / bn), rows, 2}, f32);
-    auto logit = at::empty({rows}, f32);
+    auto partial = new_tensor({2 * ((vocab + bn - 1) / bn), rows, 2}, at::kFloat, device), logit = new_tensor({rows}, at::kFloat, device);
     p.target = reinterpret_cast<const long long*>(target.data_ptr<int64_t>());
     p.partial = reinterpret_cast<float2*>(partial.data_ptr<float>());
     p.target_logit = logit.data_ptr<float>();
@@ -452,43 +449,43 @@ std::vector<Tensor> vocab_loss_fwd(const Tensor& hidden, const Tensor& weight, c
            lse2.data_ptr<float>(), loss.data_ptr<float>(), p.err);
     count_launch();
   }
-  if (reduction == 0) return {loss, lse2, out};
+  if (reduction == 0) return {loss, lse2, Tensor()};
+  auto total = new_tensor({}, at::kFloat, device), count = new_tensor({}, at::kFloat, device);
   launch(vocab_sum_kernel, 1, 1024, 0, stream, (const float*)loss.data_ptr<float>(), reinterpret_cast<const long long*>(target.data_ptr<int64_t>()), (int)rows, (int)vocab, reduction == 2,
-         out.data_ptr<float>());
+         total.data_ptr<float>(), count.data_ptr<float>());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   count_launch();
-  return {out[0], lse2, out[1]};
+  return {total, lse2, count};
 }
 
-// g: gradient of the loss ([rows] fp32 without a reduction, one element with one).  Returns {dh (bf16, or fp32 with `fp32_dh`), dW}: undefined where not wanted or, for dW,
-// where it was added to `grad` (fp32 [vocabulary, hidden], contiguous).  `workspace`: bytes that dz of one piece may take.
-std::vector<Tensor> vocab_loss_bwd(const Tensor& g, const Tensor& hidden, const Tensor& weight, const Tensor& target, const Tensor& lse2, const Tensor& count, int64_t reduction, bool want_dh,
-                                   bool fp32_dh, bool want_dw, bool fp32_dw, const c10::optional<Tensor>& grad, int64_t workspace, const Tensor& err) {
+std::pair<Tensor, Tensor> vocab_loss_bwd(const Tensor& g, const Tensor& hidden, const Tensor& weight, const Tensor& target, const Tensor& lse2, const Tensor& count, int64_t reduction,
+                                         bool want_dh, bool fp32_dh, bool want_dw, bool fp32_dw, const Tensor& grad, int64_t workspace, const Tensor& err) {
   check(hidden, weight, target);
   TORCH_CHECK(g.device() == hidden.device() && g.scalar_type() == at::kFloat && g.is_contiguous() && g.numel() == (reduction ? 1 : hidden.size(0)) && lse2.numel() == hidden.size(0),
               "vocab_loss_bwd: bad gradient");
   const c10::cuda::CUDAGuard guard(hidden.device());
   const int64_t rows = hidden.size(0), K = hidden.size(1), vocab = weight.size(0), Kp = K % 8 ? padded(K) : K;
-  const auto f32 = hidden.options().dtype(at::kFloat);
+  const auto device = hidden.device();
+  const auto dh_type = fp32_dh ? at::kFloat : at::kBFloat16, dw_type = fp32_dw ? at::kFloat : at::kBFloat16;
   auto stream = at::cuda::getCurrentCUDAStream();
   Tensor dh, dw;
   if (rows == 0) {
-    if (want_dh) dh = at::empty({0, K}, fp32_dh ? f32 : hidden.options());
-    if (want_dw && !grad.has_value()) dw = at::zeros({vocab, K}, fp32_dw ? f32 : weight.options());
+    if (want_dh) dh = new_tensor({0, K}, dh_type, device);
+    if (want_dw && !grad.defined()) dw = new_tensor({vocab, K}, dw_type, device).zero_();
     return {dh, dw};
   }
   const Tensor h = tma_rows(hidden, stream), w = tma_rows(weight, stream);
   // Pieces: as few as the workspace allows, of equal width (whole tiles)
   const int64_t widest = std::max<int64_t>(256, workspace / (2 * rows) / 256 * 256), pieces = (vocab + widest - 1) / widest;
   const int64_t width = std::min((vocab + 7) / 8 * 8, ((vocab + pieces - 1) / pieces + 255) / 256 * 256);
-  auto dz_all = at::empty({rows, width}, hidden.options());
+  auto dz_all = new_tensor({rows, width}, at::kBFloat16, device);
   // dh: where its tiles leave SMs without work, parts of the reduction side by side, added in order at the end
   const int64_t slabs = pick_slabs(rows, K, std::min(width, vocab));
   const bool direct = want_dh && slabs == 1 && pieces == 1;
   Tensor part;
-  if (want_dh && !direct) part = at::empty({slabs, rows, Kp}, f32);
-  if (direct) dh = at::empty({rows, Kp}, fp32_dh ? f32 : hidden.options());
-  if (want_dw && !grad.has_value()) dw = at::empty({vocab, Kp}, fp32_dw ? f32 : weight.options());
+  if (want_dh && !direct) part = new_tensor({slabs, rows, Kp}, at::kFloat, device);
+  if (direct) dh = new_tensor({rows, Kp}, dh_type, device);
+  if (want_dw && !grad.defined()) dw = new_tensor({vocab, Kp}, dw_type, device);
   VocabArgs p{};
   p.target = reinterpret_cast<const long long*>(target.data_ptr<int64_t>());
   p.lse2 = lse2.data_ptr<float>();
@@ -506,12 +503,12 @@ std::vector<Tensor> vocab_loss_bwd(const Tensor& g, const Tensor& hidden, const 
     if (direct) gemm_bf16_scaled(dz, wp, dh.narrow(1, 0, K), false, true, num, den, false, 0, err);
     else if (want_dh) gemm_bf16_scaled(dz, wp, part.narrow(2, 0, K), false, true, num, den, !first, slabs, err);
     if (want_dw) {
-      if (grad.has_value()) gemm_bf16_scaled(dz, h, grad->narrow(0, at, cols), true, true, num, den, true, 0, err);
+      if (grad.defined()) gemm_bf16_scaled(dz, h, grad.narrow(0, at, cols), true, true, num, den, true, 0, err);
       else gemm_bf16_scaled(dz, h, dw.narrow(0, at, cols).narrow(1, 0, K), true, true, num, den, false, 0, err);
     }
   }
   if (want_dh && !direct) {
-    dh = at::empty({rows, K}, fp32_dh ? f32 : hidden.options());
+    dh = new_tensor({rows, K}, dh_type, device);
     auto kernel = fp32_dh ? vocab_slabs_kernel<false> : vocab_slabs_kernel<true>;
     launch(kernel, (unsigned)std::min<int64_t>((rows + 7) / 8, kNumSMs * 8), 256, 0, stream, (const float*)part.data_ptr<float>(), (int)slabs, (long long)(rows * Kp), (int)rows, (int)K, (int)Kp,
            dh.data_ptr());
@@ -519,12 +516,12 @@ std::vector<Tensor> vocab_loss_bwd(const Tensor& g, const Tensor& hidden, const 
     count_launch();
   } else if (direct && Kp != K) {
     const Tensor wide = dh.narrow(1, 0, K);
-    dh = at::empty({rows, K}, wide.options());
+    dh = new_tensor({rows, K}, dh_type, device);
     copy_rows(wide, dh, stream);
   }
   if (dw.defined() && Kp != K) {
     const Tensor wide = dw.narrow(1, 0, K);
-    dw = at::empty({vocab, K}, wide.options());
+    dw = new_tensor({vocab, K}, dw_type, device);
     copy_rows(wide, dw, stream);
   }
   return {dh, dw};

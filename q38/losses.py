@@ -17,6 +17,7 @@ import torch
 import torch.nn.functional as F
 
 from .models import RouterStats, modeling
+from .ops.vocab import vocabulary_loss
 
 
 def linear_cross_entropy(weight, hidden, target, reduction="mean"):
@@ -40,6 +41,8 @@ def vocabulary_cross_entropy(weight, hidden, target, reduction="mean"):
     products for memory that does not grow with the vocabulary."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"vocabulary_cross_entropy: reduction must be mean, sum or none, got {reduction!r}")
+    if hidden.is_cuda:
+        return vocabulary_loss(hidden, weight, target, reduction)
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1] or not weight.numel():
         raise ValueError("vocabulary_cross_entropy: hidden [..., h] and weight [vocabulary, h] required")
     if target.shape != hidden.shape[:-1] or target.dtype != torch.int64:
@@ -49,10 +52,6 @@ def vocabulary_cross_entropy(weight, hidden, target, reduction="mean"):
     if weight.device != hidden.device or target.device != hidden.device:
         raise ValueError("vocabulary_cross_entropy: hidden, weight and target on one device required")
     h2, t1 = hidden.reshape(-1, hidden.shape[-1]), target.reshape(-1)
-    if hidden.is_cuda:
-        from .ops.vocab import vocabulary_loss
-        loss = vocabulary_loss(h2, weight, t1.contiguous(), reduction)
-        return loss.view(target.shape) if reduction == "none" else loss
     scores = F.linear(h2, weight.to(h2.dtype)).float()
     losses = F.cross_entropy(scores, t1, ignore_index=-100, reduction="none")
     if reduction == "none":

@@ -24,6 +24,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
     x: fp32, bf16 or fp16, any leading dimensions and strides.  weight, bias: vectors of the last dimension's length in any of these types, either may be
     absent.  The result has x's type, or bf16 (`out_dtype`) for an fp32 x.  Gradients of x, weight and bias come in their types; the sums over rows
     are fp32 and have the same bits in every run."""
+    if x.is_cuda:                                # checked there
+        return load().layer_norm(x, weight, bias, eps, out_dtype)
     dim = x.shape[-1] if x.dim() else 0
     _require(dim > 0, "layer_norm: an input with a last dimension that is not empty is required")
     _require(x.dtype in FLOATS, f"layer_norm: fp32, bf16 or fp16 input required, got {x.dtype}")
@@ -34,8 +36,6 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out_dtype=None):
         if p is not None:
             _require(p.dim() == 1 and p.shape[0] == dim and p.device == x.device and p.dtype in FLOATS,
                      "layer_norm: weight and bias are fp32, bf16 or fp16 vectors of the last dimension's length on the input's device")
-    if x.is_cuda:
-        return load().layer_norm(x, weight, bias, eps, out_dtype)
     xf = x.float()
     centred = xf - xf.mean(-1, keepdim=True)
     y = centred * torch.rsqrt(centred.square().mean(-1, keepdim=True) + eps)
@@ -107,6 +107,9 @@ def rotary(q, k, positions, frequencies, magnitude=1.0, interleaved=False):
         _require(k is None or k.dim() == 3, "rotary: queries and keys have the same number of dimensions")
         q2, k2 = rotary(q.unsqueeze(0), None if k is None else k.unsqueeze(0), positions, frequencies, magnitude, interleaved)
         return q2.squeeze(0), None if k2 is None else k2.squeeze(0)
+    if q.is_cuda:                                # checked there
+        out = load().rotary(q, k, positions, frequencies, magnitude, interleaved)
+        return out if k is not None else (out[0], None)
     _require(q.dim() == 4 and q.dtype in FLOATS, "rotary: fp32, bf16 or fp16 queries [batch, seq, heads, dim] required")
     B, S, _, D = q.shape
     if k is not None:
@@ -116,9 +119,6 @@ def rotary(q, k, positions, frequencies, magnitude=1.0, interleaved=False):
              "rotary: whole positions [seq] or [batch, seq] on the queries' device required")
     _require(frequencies.dtype == torch.float64 and frequencies.device == q.device and frequencies.dim() == 1 and 2 * frequencies.shape[0] <= D,
              "rotary: 64-bit frequencies on the queries' device, at most half a head of them, required")
-    if q.is_cuda:
-        out = load().rotary(q, k, positions, frequencies.contiguous(), float(magnitude), interleaved)
-        return out[0], out[1] if k is not None else None
     angle = positions.double()[..., None, None] * frequencies
     cos, sin = (angle.cos() * magnitude).float(), (angle.sin() * magnitude).float()
     return _rotate(q, cos, sin, interleaved), None if k is None else _rotate(k, cos, sin, interleaved)
@@ -126,6 +126,8 @@ def rotary(q, k, positions, frequencies, magnitude=1.0, interleaved=False):
 
 # ---- gradient norm and clipping ------------------------------------------------------------------------------------------------------
 def _gradients(grads, out=None):
+    if type(grads) is list and (out is None or type(out) is list and len(out) == len(grads)) and grads and all([g is not None for g in grads]):
+        return grads, out
     grads = [grads] if torch.is_tensor(grads) else list(grads)
     if out is not None:
         out = [out] if torch.is_tensor(out) else list(out)

@@ -1,7 +1,4 @@
-"""Cross entropy of a vocabulary projection in pieces of the vocabulary (`csrc/vocab_loss.cu`): the autograd node behind `q38.losses.vocabulary_cross_entropy`."""
-import torch
-from torch.autograd.function import once_differentiable
-
+"""Cross entropy of a vocabulary projection in pieces of the vocabulary (`csrc/vocab_loss.cu`), behind `q38.losses.vocabulary_cross_entropy`."""
 from . import error_flag, load
 from .backend import _bf16_weight
 
@@ -11,35 +8,8 @@ PIECE_BYTES = 256 << 20
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
 
-class _VocabularyLoss(torch.autograd.Function):
-    """Keeps the hidden states, the weight, the targets and one number per row; the backward forms the scores again, piece by piece."""
-
-    @staticmethod
-    def forward(ctx, hidden, weight, target, reduction):
-        h = hidden if hidden.dtype == torch.bfloat16 else hidden.to(torch.bfloat16)
-        loss, lse, count = load().vocab_loss_fwd(h, _bf16_weight(weight), target, reduction, error_flag(h.device))
-        ctx.save_for_backward(h, weight, target, lse, count)
-        ctx.reduction, ctx.dtype = reduction, hidden.dtype
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        h, weight, target, lse, count = ctx.saved_tensors
-        want_dh, want_dw = ctx.needs_input_grad[:2]
-        # a parameter of the trainer's arena has its gradient added in place; any other gets it returned
-        grad = weight.grad if want_dw and getattr(weight, "_q38_bf16", None) is not None else None
-        if grad is not None and (grad.dtype != torch.float32 or not grad.is_contiguous() or grad.shape[1] % 4 or grad.data_ptr() % 16):
-            grad = None
-        dh, dw = load().vocab_loss_bwd(g.float().contiguous(), h, _bf16_weight(weight), target, lse, count, ctx.reduction, want_dh, ctx.dtype == torch.float32, want_dw,
-                                       weight.dtype == torch.float32, grad, PIECE_BYTES, error_flag(h.device))
-        return dh, dw, None, None
-
-
 def vocabulary_loss(hidden, weight, target, reduction):
-    """hidden [rows, h], weight [vocabulary, h], target [rows] on one GPU; `reduction` a key of REDUCTIONS."""
-    code = REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        return _VocabularyLoss.apply(hidden, weight, target, code)
-    h = hidden if hidden.dtype == torch.bfloat16 else hidden.to(torch.bfloat16)
-    return load().vocab_loss_fwd(h, _bf16_weight(weight), target, code, error_flag(h.device))[0]
+    """hidden [..., h], weight [vocabulary, h], target [...] on one GPU; `reduction` a key of REDUCTIONS.  A parameter of the trainer's arena (it carries its bf16
+    shadow) has its gradient added to its buffer in place, any other gets it returned."""
+    managed = getattr(weight, "_q38_bf16", None) is not None
+    return load().vocab_loss(hidden, weight, _bf16_weight(weight), target, REDUCTIONS[reduction], managed, PIECE_BYTES, error_flag(hidden.device))
