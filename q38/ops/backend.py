@@ -807,6 +807,7 @@ class Backend:
         self.ep = None            # an `ExpertParallel` context when the experts are split over ranks
         self.selection_override = None   # optional iterator of (count, index) pairs that replaces the block selection (tests)
         self.fp8_ffn = False      # routed experts on block-scaled MXFP8 GEMMs (`q38.ops.fp8`); set by the trainer from --fp8_ffn
+        self.ce_pieces = False    # vocabulary losses in pieces of the vocabulary (`q38.ops.vocab`); set by the trainer from --ce_pieces
         if self_check:
             self._self_check()
 
@@ -1094,7 +1095,11 @@ class Backend:
 
     @_nvtx("q38.linear_cross_entropy")
     def linear_cross_entropy(self, weight, hidden, target, reduction):
-        """Chunked logits + CE; logits of one chunk only ever exist, in fp32."""
+        """Chunked logits + CE; logits of one chunk only ever exist, in fp32.  With `ce_pieces` the loss is formed in pieces of the vocabulary instead and
+        no logits are kept for the backward."""
+        if self.ce_pieces:
+            from .vocab import vocabulary_loss
+            return vocabulary_loss(hidden, weight, target, reduction)
         return _chunked_linear_ce(self, weight, hidden, target, reduction)
 
     def describe(self):

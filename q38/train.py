@@ -52,7 +52,7 @@ TRAIN_DEFAULTS = dict(
     eval_sampling="random", eval_offset=0, final_eval_tokens=0, final_eval_offset=0, require_ready_pool=0,
     auto_micro_bs=0, probe_mem_frac=0.92, mtp_coef=0.3, kl_coef=0.05, muon=1, dense_warmup=1, grad_ckpt=0)
 # Options of this framework that the reference trainer does not have (never part of the resume contract).
-ENGINE_DEFAULTS = dict(grad_sync="auto", fp8_ffn=0, expert_parallel=0, ep_capacity=4.0, export_hf=1, device="auto", cuda_graphs=1, overlap_wgrad=1)
+ENGINE_DEFAULTS = dict(grad_sync="auto", fp8_ffn=0, expert_parallel=0, ep_capacity=4.0, export_hf=1, device="auto", cuda_graphs=1, overlap_wgrad=1, ce_pieces=0)
 
 # Everything that shapes the model, the data stream or the schedule must be unchanged on resume.
 RESUME_KEYS = (
@@ -120,6 +120,7 @@ def parse_args(argv=None):
         (a.data_seed >= -1, "data_seed must be -1 (use model seed) or nonnegative"),
         (a.grad_sync in ("auto", "p2p", "collective"), "--grad_sync must be auto, p2p or collective"),
         (a.fp8_ffn in (0, 1) and not (a.fp8_ffn and a.expert_parallel), "--fp8_ffn must be 0 or 1 and cannot be combined with --expert_parallel 1"),
+        (a.ce_pieces in (0, 1), "--ce_pieces must be 0 or 1"),
         (not a.fp8_ffn or (a.hidden % 16 == 0 and a.moe_ffn % 16 == 0), "--fp8_ffn 1 needs hidden and moe_ffn to be multiples of 16"),
     ]
     for ok, message in checks:
@@ -359,6 +360,7 @@ class Trainer:
         if dev.type == "cuda":
             from .models import modeling
             modeling.get_backend().fp8_ffn = bool(getattr(a, "fp8_ffn", 0))      # routed experts on block-scaled MXFP8 GEMMs
+            modeling.get_backend().ce_pieces = bool(getattr(a, "ce_pieces", 0))  # vocabulary losses piece by piece: no scores kept for the backward
         self.model.train()
         # One CUDA graph per (micro-batch shape, accumulation count, attention phase) replays forward + backward of a
         # micro-step without any per-kernel host work; the optimizer step stays eager.
@@ -386,6 +388,7 @@ class Trainer:
             backend.ep = None
         if backend is not None:
             backend.fp8_ffn = False
+            backend.ce_pieces = False
             if self.dev.type == "cuda":
                 from .ops import fp8
                 fp8.drop_weights()

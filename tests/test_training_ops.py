@@ -159,3 +159,11 @@ def test_vocabulary_loss_refuses(wrong):
     _vocab()
     with pytest.raises(ValueError):
         _vocab(**wrong)
+
+
+def test_trainer_flag_for_the_loss_in_pieces():
+    from q38.train import parse_args
+    assert parse_args(["--preset", "q38_c2"]).ce_pieces == 0
+    assert parse_args(["--preset", "q38_c2", "--ce_pieces", "1"]).ce_pieces == 1
+    with pytest.raises(SystemExit):
+        parse_args(["--preset", "q38_c2", "--ce_pieces", "2"])
