@@ -163,7 +163,7 @@ def test_vocabulary_loss_refuses(wrong):
 
 def test_trainer_flag_for_the_loss_in_pieces():
     from q38.train import parse_args
-    assert parse_args(["--preset", "q38_c2"]).ce_pieces == 0
-    assert parse_args(["--preset", "q38_c2", "--ce_pieces", "1"]).ce_pieces == 1
+    common = ["--run_dir", "runs/x", "--tokens", "100000"]
+    assert parse_args(common).ce_pieces == 0 and parse_args(common + ["--ce_pieces", "1"]).ce_pieces == 1
     with pytest.raises(SystemExit):
-        parse_args(["--preset", "q38_c2", "--ce_pieces", "2"])
+        parse_args(common + ["--ce_pieces", "2"])
