@@ -135,7 +135,11 @@ namespace {
 
 using at::Tensor;
 
-Tensor like(const Tensor& t) { return t.is_contiguous() ? new_tensor(t.sizes(), t.scalar_type(), t.device()) : at::empty_like(t); }
+// A tensor of t's shape with its order of dimensions in memory
+Tensor like(const Tensor& t) {
+  const bool in_order = t.stride(0) >= t.stride(1) && t.stride(1) >= t.stride(2) && t.stride(2) >= t.stride(3);
+  return in_order ? new_tensor(t.sizes(), t.scalar_type(), t.device()) : at::empty_like(t);
+}
 Tensor with_columns(const Tensor& t) { return t.stride(3) == 1 || t.size(3) == 1 ? t : t.contiguous(); }
 
 RotarySide side_of(const Tensor& in, const Tensor& out) {
@@ -202,7 +206,7 @@ std::pair<Tensor, Tensor> rotary_apply(const Tensor& q_in, const Tensor& k_in, c
   p.freq = freq.data_ptr<double>(); p.pos = pos.data_ptr(); p.pos64 = pos.scalar_type() == at::kLong;
   p.pos_b = pos.dim() == 2 && pos.size(0) > 1 ? pos.stride(0) : 0; p.pos_s = pos.stride(-1);
   p.magnitude = (float)magnitude; p.sign = (float)sign;
-  if (p.tokens > 0 && p.heads.d > 0) {
+  if (p.tokens > 0 && p.heads.d > 0 && p.dim > 0) {
     auto stream = at::cuda::getCurrentCUDAStream();
     if (any.scalar_type() == at::kBFloat16) by_width<__nv_bfloat16>(p, fit, interleaved, stream);
     else if (any.scalar_type() == at::kHalf) by_width<__half>(p, fit, interleaved, stream);

@@ -158,7 +158,8 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weig
     auto node = std::shared_ptr<VocabLossBackward>(new VocabLossBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(hidden, weight));
     node->hidden = SavedVariable(h16, false);
-    node->weight = SavedVariable(weight16, false);
+    // a copy that was made in inference mode cannot be saved
+    node->weight = SavedVariable(weight16.is_inference() ? weight.detach().to(at::kBFloat16) : weight16, false);
     node->target = SavedVariable(t, false);
     node->lse2 = lse2; node->count = count; node->err = err;
     if (managed) node->parameter = weight;

@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(V_THREADS) vocab_tiles_kernel(const __grid_con
       auto use = [&](uint32_t (&r)[32], int c0) { if constexpr (GRAD) emit(r, c0); else reduce(r, c0); };
       uint32_t ra[32], rb[32];
       int c0 = 32 * group;
-      ptx::tmem_ld_32x32b_x32(t_addr + c0, ra);                    // bn is a multiple of 64: every warp has a chunk
+      ptx::tmem_ld_32x32b_x32(t_addr + c0, ra);                    // bn is 64 at least: every warp has a chunk
       for (; c0 < p.bn; c0 += 128) {                               // two chunks of this warpgroup per trip, the next one's read in flight
         ptx::tmem_ld_wait();
         if (c0 + 64 < p.bn) ptx::tmem_ld_32x32b_x32(t_addr + c0 + 64, rb);
@@ -364,7 +364,7 @@ int64_t padded(int64_t n) { return (n + 63) / 64 * 64; }
 // (rows 16 bytes off a line cost two lines per box: 2049 x 30011 x 711, the tiles' kernel 109 -> 71 us)
 Tensor tma_rows(const Tensor& t, cudaStream_t stream) {
   const int64_t n = t.size(1);
-  if ((t.stride(1) == 1 || n == 1) && (t.stride(0) >= n || t.size(0) == 1) && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) return t;
+  if ((t.stride(1) == 1 || n == 1) && t.stride(0) >= n && t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0) return t;
   auto view = new_tensor({t.size(0), padded(n)}, t.scalar_type(), t.device()).narrow(1, 0, n);
   copy_rows(t, view, stream);
   return view;
@@ -433,21 +433,27 @@ std::array<Tensor, 3> vocab_loss_fwd(const Tensor& hidden, const Tensor& weight,
   const auto device = hidden.device();
   const c10::cuda::CUDAGuard guard(device);
   const int64_t rows = hidden.size(0), vocab = weight.size(0);
-  auto loss = new_tensor(reduction ? at::IntArrayRef(rows) : shape, at::kFloat, device), lse2 = new_tensor({rows}, at::kFloat, device);
+  auto loss = new_tensor(reduction ? at::IntArrayRef(&rows, 1) : shape, at::kFloat, device), lse2 = new_tensor({rows}, at::kFloat, device);
   auto stream = at::cuda::getCurrentCUDAStream();
   if (rows) {
-    const Tensor h = tma_rows(hidden, stream), w = tma_rows(weight, stream);
-    VocabArgs p{};
-    const int bn = tile_width(rows, vocab);
-    auto partial = new_tensor({2 * ((vocab + bn - 1) / bn), rows, 2}, at::kFloat, device), logit = new_tensor({rows}, at::kFloat, device);
-    p.target = reinterpret_cast<const long long*>(target.data_ptr<int64_t>());
-    p.partial = reinterpret_cast<float2*>(partial.data_ptr<float>());
-    p.target_logit = logit.data_ptr<float>();
-    p.err = err.data_ptr<int>();
-    launch_tiles<false>(h, w, 0, vocab, p, nullptr, stream);
-    launch(vocab_join_kernel, (unsigned)((rows + 31) / 32), 1024, 0, stream, (const float2*)p.partial, 2 * p.tiles_n, (int)rows, (int)vocab, p.target, (const float*)p.target_logit,
-           lse2.data_ptr<float>(), loss.data_ptr<float>(), p.err);
-    count_launch();
+    const Tensor w = tma_rows(weight, stream);
+    // 65536 rows at a time bound the pairs' workspace (a sixteenth of a byte per row and column)
+    for (int64_t at = 0; at < rows; at += 65536) {
+      const int64_t n = std::min<int64_t>(65536, rows - at);
+      const Tensor h = tma_rows(hidden.narrow(0, at, n), stream);
+      VocabArgs p{};
+      const int bn = tile_width(n, vocab);
+      auto partial = new_tensor({2 * ((vocab + bn - 1) / bn), n, 2}, at::kFloat, device), logit = new_tensor({n}, at::kFloat, device);
+      p.target = reinterpret_cast<const long long*>(target.data_ptr<int64_t>()) + at;
+      p.partial = reinterpret_cast<float2*>(partial.data_ptr<float>());
+      p.target_logit = logit.data_ptr<float>();
+      p.err = err.data_ptr<int>();
+      launch_tiles<false>(h, w, 0, vocab, p, nullptr, stream);
+      launch(vocab_join_kernel, (unsigned)((n + 31) / 32), 1024, 0, stream, (const float2*)p.partial, 2 * p.tiles_n, (int)n, (int)vocab, p.target, (const float*)p.target_logit,
+             lse2.data_ptr<float>() + at, loss.data_ptr<float>() + at, p.err);
+      C10_CUDA_KERNEL_LAUNCH_CHECK();
+      count_launch();
+    }
   }
   if (reduction == 0) return {loss, lse2, Tensor()};
   auto total = new_tensor({}, at::kFloat, device), count = new_tensor({}, at::kFloat, device);

@@ -403,3 +403,49 @@ def test_training_ops_replay_from_a_graph_and_run_on_another_stream():
         torch.cuda.synchronize()
         assert all(torch.equal(a, e) for a, e in zip(held, step()))
     assert all(t.isfinite().all() for t in other)
+
+
+def test_rotary_of_empty_heads():
+    f = torch.zeros(0, device="cuda", dtype=torch.float64)
+    x = torch.zeros(1, 2, 3, 0, device="cuda")
+    assert ops.rotary(x, None, torch.zeros(2, device="cuda", dtype=torch.int64), f)[0].shape == x.shape
+    q, k = torch.zeros(1, 2, 0, 8, device="cuda"), torch.ones(1, 2, 1, 8, device="cuda")
+    qo, ko = ops.rotary(q, k, torch.zeros(2, device="cuda", dtype=torch.int64), ops.rotary_frequencies(8, device="cuda")[0])
+    assert qo.shape == q.shape and torch.equal(ko, k)
+
+
+@pytest.mark.parametrize("call", [
+    lambda c: ops.layer_norm(c(3, 0)), lambda c: ops.layer_norm(c(3, 4, dtype=torch.float64)), lambda c: ops.layer_norm(c(3, 4), c(3)), lambda c: ops.layer_norm(c(3, 4), torch.ones(4)),
+    lambda c: ops.layer_norm(c(3, 4), eps=-1.0), lambda c: ops.layer_norm(c(3, 4, dtype=BF16), out_dtype=FP32), lambda c: ops.layer_norm(c(3, 4), None, c(4, 1)),
+    lambda c: ops.rotary(c(1, 2, 3, 8), None, torch.zeros(2, dtype=torch.int64), c(4, dtype=torch.float64)), lambda c: ops.rotary(c(1, 2, 3, 8), None, c(2, dtype=torch.int64), c(4)),
+    lambda c: ops.rotary(c(1, 2, 3, 8), c(1, 2, 3, 6), c(2, dtype=torch.int64), c(4, dtype=torch.float64)), lambda c: ops.rotary(c(1, 2, 3, 8), None, c(3, dtype=torch.int64), c(4, dtype=torch.float64)),
+    lambda c: ops.rotary(c(1, 2, 3, 8), None, c(2, dtype=torch.int64), c(5, dtype=torch.float64)), lambda c: ops.rotary(c(1, 2, 3, 8, dtype=torch.float64), None, c(2, dtype=torch.int64), c(4, dtype=torch.float64)),
+    lambda c: ops.grad_norm([]), lambda c: ops.grad_norm([c(3, dtype=torch.int64)]),
+])
+def test_refusals_on_the_gpu(call):
+    with pytest.raises(ValueError):
+        call(lambda *shape, **kw: torch.zeros(*shape, device="cuda", **kw))
+
+
+def test_operators_in_two_threads():
+    """Calls at once from two threads, on a stream each."""
+    import threading
+    x, g = torch.randn(512, 640, device="cuda"), [torch.randn(3000, device="cuda") for _ in range(70)]
+    f = ops.rotary_frequencies(64, device="cuda")[0]
+    pos, results = torch.arange(512, device="cuda"), {}
+    torch.cuda.synchronize()
+
+    def work(who):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                leaf = x.clone().requires_grad_()
+                y = ops.layer_norm(leaf)
+                q, _ = ops.rotary(y.view(512, 10, 64), None, pos, f)
+                d, = torch.autograd.grad(q, leaf, torch.ones_like(q))
+                results[who] = (q.detach(), d, ops.clip_grad_norm(g, 1.0, out=[torch.empty_like(t) for t in g]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert all(torch.equal(a, b) for a, b in zip(results[0], results[1]))

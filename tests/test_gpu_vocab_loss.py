@@ -264,3 +264,29 @@ def test_replay_from_a_graph_and_another_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, step()))
+
+
+def test_more_rows_than_one_pass_takes():
+    h, w, target = inputs(65536 + 300, 300, 16, seed=14)
+    check(h, w, target, "none")
+
+
+def test_training_after_inference_mode():
+    h, w, target = inputs(50, 400, 64, seed=15)
+    master = w.float().requires_grad_()
+    with torch.inference_mode():
+        seen = vocabulary_cross_entropy(master, h, target)           # leaves a bf16 copy of the weight behind
+    loss = vocabulary_cross_entropy(master, h, target)
+    assert torch.equal(loss, seen) and torch.autograd.grad(loss, master)[0].isfinite().all()
+
+
+def test_changes_before_the_backward_are_noticed():
+    for what in range(3):
+        h, w, target = inputs(50, 400, 64, seed=16)
+        leaf, other = h.clone().requires_grad_(), w.clone().requires_grad_()
+        mid, mid_w = leaf * 1.0, other * 1.0
+        loss = vocabulary_cross_entropy(mid_w, mid, target)
+        with torch.no_grad():
+            (mid, mid_w, target)[what].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
