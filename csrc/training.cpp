@@ -122,15 +122,16 @@ struct VocabLossBackward : public Node {
     const std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("vocabulary_cross_entropy");
     if (!grads[0].defined()) return variable_list(2);
-    const Tensor h = hidden.unpack(), w = weight.unpack(), t = target.unpack(), g = grads[0].reshape({-1}).to(at::kFloat).contiguous();
+    const Tensor h = hidden.unpack(), w = weight.unpack(), t = target.unpack();
+    const Tensor g = grads[0].scalar_type() == at::kFloat && grads[0].is_contiguous() ? grads[0] : grads[0].to(at::kFloat).contiguous();
     const bool want_dw = task_should_compute_output(1);
     Tensor buffer;
     if (want_dw && parameter.defined()) {
       const Tensor& own = parameter.grad();
       if (own.defined() && own.scalar_type() == at::kFloat && own.is_contiguous() && own.size(1) % 4 == 0 && (reinterpret_cast<uintptr_t>(own.data_ptr()) & 15) == 0) buffer = own;
     }
-    auto out = vocab_loss_bwd(g, h.view({-1, w.size(1)}), w, t.view({-1}), lse2, count, reduction, task_should_compute_output(0), fp32_dh, want_dw, fp32_dw, buffer, workspace, err);
-    return {out.first.defined() ? out.first.view(shape) : out.first, out.second};
+    auto out = vocab_loss_bwd(g, h.dim() == 2 ? h : h.view({-1, w.size(1)}), w, t.dim() == 1 ? t : t.view({-1}), lse2, count, reduction, task_should_compute_output(0), fp32_dh, want_dw, fp32_dw, buffer, workspace, err);
+    return {out.first.defined() && shape.size() != 2 ? out.first.view(shape) : out.first, out.second};
   }
 };
 

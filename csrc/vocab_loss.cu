@@ -358,6 +358,9 @@ void copy_rows(const Tensor& in, const Tensor& out, cudaStream_t stream) {
   count_launch();
 }
 
+// The first n columns (views cost the host as much as launches: none where all are meant)
+Tensor columns(const Tensor& t, int64_t n) { return t.size(-1) == n ? t : t.narrow(-1, 0, n); }
+
 int64_t padded(int64_t n) { return (n + 63) / 64 * 64; }
 
 // A 2-D bf16 tensor whose rows TMA accepts (contiguous, a multiple of 16 bytes apart, on 16 bytes); others are copied into rows of whole 128-byte lines
@@ -440,7 +443,7 @@ std::array<Tensor, 3> vocab_loss_fwd(const Tensor& hidden, const Tensor& weight,
     // 65536 rows at a time bound the pairs' workspace (a sixteenth of a byte per row and column)
     for (int64_t at = 0; at < rows; at += 65536) {
       const int64_t n = std::min<int64_t>(65536, rows - at);
-      const Tensor h = tma_rows(hidden.narrow(0, at, n), stream);
+      const Tensor h = tma_rows(n == rows ? hidden : hidden.narrow(0, at, n), stream);
       VocabArgs p{};
       const int bn = tile_width(n, vocab);
       auto partial = new_tensor({2 * ((vocab + bn - 1) / bn), n, 2}, at::kFloat, device), logit = new_tensor({n}, at::kFloat, device);
@@ -505,12 +508,12 @@ std::pair<Tensor, Tensor> vocab_loss_bwd(const Tensor& g, const Tensor& hidden, 
     const bool first = at == 0;
     const CUtensorMap tc = make_tmap_box(dz_all.data_ptr(), 2, cols, rows, 1, width, 0, 32, 64);
     launch_tiles<true>(h, w, at, cols, p, &tc, stream);
-    const Tensor dz = dz_all.narrow(1, 0, cols), wp = w.narrow(0, at, cols);
-    if (direct) gemm_bf16_scaled(dz, wp, dh.narrow(1, 0, K), false, true, num, den, false, 0, err);
-    else if (want_dh) gemm_bf16_scaled(dz, wp, part.narrow(2, 0, K), false, true, num, den, !first, slabs, err);
+    const Tensor dz = columns(dz_all, cols), wp = cols == vocab ? w : w.narrow(0, at, cols);
+    if (direct) gemm_bf16_scaled(dz, wp, columns(dh, K), false, true, num, den, false, 0, err);
+    else if (want_dh) gemm_bf16_scaled(dz, wp, columns(part, K), false, true, num, den, !first, slabs, err);
     if (want_dw) {
-      if (grad.defined()) gemm_bf16_scaled(dz, h, grad.narrow(0, at, cols), true, true, num, den, true, 0, err);
-      else gemm_bf16_scaled(dz, h, dw.narrow(0, at, cols).narrow(1, 0, K), true, true, num, den, false, 0, err);
+      if (grad.defined()) gemm_bf16_scaled(dz, h, cols == vocab ? grad : grad.narrow(0, at, cols), true, true, num, den, true, 0, err);
+      else gemm_bf16_scaled(dz, h, columns(cols == vocab ? dw : dw.narrow(0, at, cols), K), true, true, num, den, false, 0, err);
     }
   }
   if (want_dh && !direct) {

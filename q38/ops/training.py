@@ -166,20 +166,20 @@ def grad_norm(grads):
     return torch.stack([g.detach().double().square().sum() for g in grads]).sum().sqrt().float()
 
 
-@torch.no_grad()
 def clip_grad_norm(grads, max_norm, out=None):
     """Scale tensors by ``min(1, max_norm / (norm + 1e-6))`` with their global 2-norm, which is returned (before clipping, 0-dim fp32).
 
     In place, or into `out`: as many tensors of the same types, shapes and layouts (the views of an optimizer's flat buffer, say), each
     its own gradient or apart from all of them.  No tensor may be listed twice.  Where the factor is 1, nothing is written in place.  The device is not
     waited for: a norm that is not finite shows in the result and makes the scaled values NaN or zero, as the formula says."""
-    _require(max_norm > 0, "clip_grad_norm: max_norm must be positive")
     grads, out = _gradients(grads, out)
-    if grads[0].is_cuda:
+    if grads[0].is_cuda:                         # checked there
         return load().clip_grad_norm_(grads, max_norm) if out is None else load().clip_grad_norm_out(grads, out, max_norm)
+    _require(max_norm > 0, "clip_grad_norm: max_norm must be positive")
     _check_host(grads, out)
-    norm = grad_norm(grads)
-    factor = (max_norm / (norm + 1e-6)).clamp(max=1.0)
-    for o, g in zip(grads if out is None else out, grads):
-        o.copy_(g.float() * factor)
+    with torch.no_grad():
+        norm = grad_norm(grads)
+        factor = (max_norm / (norm + 1e-6)).clamp(max=1.0)
+        for o, g in zip(grads if out is None else out, grads):
+            o.copy_(g.float() * factor)
     return norm
