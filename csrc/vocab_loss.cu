@@ -303,10 +303,13 @@ __global__ void __launch_bounds__(256) vocab_slabs_kernel(const float* __restric
     const float* in = part + r * ldp;
 #pragma unroll 2
     for (int c = lane * 4; c < cols; c += 128) {                 // the last pack may end in a row's padding, which is read and not used
-      float4 s = *reinterpret_cast<const float4*>(in + c);
-      for (int k = 1; k < slabs; ++k) {
-        const float4 v = *reinterpret_cast<const float4*>(in + k * slab + c);
-        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k0 = 0; k0 < slabs; k0 += 4) {                     // four reads in flight
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = k0 + k < slabs ? *reinterpret_cast<const float4*>(in + (k0 + k) * slab + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w; }
       }
       const long long at = r * cols + c;
       if (packs) {

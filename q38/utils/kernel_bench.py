@@ -1,7 +1,7 @@
 """Per-kernel benchmark at the shapes of a preset: device time (CUDA events), achieved FLOP/s or bytes/s and the
 fraction of the measured roofline.
 
-  python -m q38.utils.kernel_bench --preset q38_c2 [--kernels gemm,moe,mhc,gdn,qsa,conv,fp8,muon,ce,ngram] [--iters 20] [--json out.json]
+  python -m q38.utils.kernel_bench --preset q38_c2 [--kernels gemm,moe,mhc,gdn,qsa,conv,fp8,muon,ce,ngram,training] [--iters 20] [--json out.json]
 
 Denominators come from ``MEASURED_PEAKS.json`` at the repository root when present (copy bandwidth and cuBLAS bf16
 throughput measured on the same pool), otherwise 6.65 TB/s and 1.59 PFLOP/s.  Inputs are larger than the 126 MB L2 or
@@ -298,6 +298,39 @@ def bench_ngram(rows, shape, T, iters, pk, seq=4096):
     report(rows, f"ngram_bwd T={T} h={h}", t, bytes_=T * h * (2.0 + 2 * 4 + 2 * 8), pk=pk)
 
 
+def bench_training(rows, shape, T, iters, pk):
+    """Layer norm, rotary positions, gradient clipping and the vocabulary loss in pieces, as `q38.ops` and `q38.losses` offer them (forward passes)."""
+    from .. import ops
+    from ..losses import vocabulary_cross_entropy
+    h, heads, kv = shape["hidden"], shape["heads"], shape["kv_heads"]
+    x = [torch.randn(T, h, device="cuda").to(torch.bfloat16) for _ in range(8)]
+    w, b = torch.ones(h, device="cuda"), torch.zeros(h, device="cuda")
+    state = {"i": 0}
+
+    def turn(items):
+        state["i"] += 1
+        return items[state["i"] % len(items)]
+
+    t = timeit(lambda: ops.layer_norm(turn(x), w, b), iters)
+    report(rows, f"layer_norm T={T} h={h}", t, bytes_=4.0 * T * h, pk=pk)
+    qkv = [torch.randn(T // 4096, 4096, heads + 2 * kv, 64, device="cuda").to(torch.bfloat16) for _ in range(4)]
+    pos, (freq, magnitude) = torch.arange(4096, device="cuda"), ops.rotary_frequencies(16, shape["rope_theta"], device="cuda")
+
+    def rotate():
+        packed = turn(qkv)
+        ops.rotary(packed[:, :, :heads], packed[:, :, heads:heads + kv], pos, freq, magnitude)
+
+    t = timeit(rotate, iters)
+    report(rows, f"rotary T={T} heads={heads}+{kv}", t, bytes_=4.0 * (T // 4096 * 4096) * (heads + kv) * 64, pk=pk)
+    grads = [torch.randn(2_000_000, device="cuda") for _ in range(60)]
+    out = [torch.empty_like(g) for g in grads]
+    t = timeit(lambda: ops.clip_grad_norm(grads, 1.0, out=out), iters)
+    report(rows, "clip_grad_norm 60 x 2e6 fp32", t, bytes_=12.0 * sum(g.numel() for g in grads), pk=pk)
+    weight, target = torch.randn(50048, h, device="cuda").mul_(h ** -0.5).to(torch.bfloat16), torch.randint(0, 50048, (T,), device="cuda")
+    t = timeit(lambda: vocabulary_cross_entropy(weight, turn(x), target), iters)
+    report(rows, f"vocabulary_cross_entropy T={T} V=50048 h={h}", t, flops=2.0 * T * 50048 * h, pk=pk)
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--preset", default="q38_c2")
@@ -313,7 +346,7 @@ def main(argv=None):
     pk = peaks()
     rows = []
     torch.manual_seed(0)
-    BENCHES.update(fp8=bench_fp8, muon=bench_muon, ce=bench_ce, ngram=bench_ngram)
+    BENCHES.update(fp8=bench_fp8, muon=bench_muon, ce=bench_ce, ngram=bench_ngram, training=bench_training)
     for name in a.kernels.split(","):
         BENCHES[name](rows, shape, a.tokens, a.iters, pk)
     ops.check_errors()
