@@ -489,10 +489,10 @@ void launch_fwd(LnArgs& p, cudaStream_t stream) {
 }
 
 struct BwdShape { int G, groups, ctas; };
-// Elements per thread: eight or sixteen.  The sums over a group cost some sixty instructions per thread and row, so packed rows, which have the registers, take sixteen.
+// Elements per thread: eight, or more.  The sums over a group cost some sixty instructions per thread and row, so packed rows, which have the registers, take sixteen or thirty-two.
 bool eight_each(int dim, bool packed16) { return dim <= 256 || (!packed16 && dim > 512 && dim <= 4096); }
 
-// Threads per row, rows per CTA and CTAs.  Eight 16-bit elements per thread take 64 registers (1024 threads per SM), eight others up to 96 (640), sixteen up to 128 (512);
+// Threads per row, rows per CTA and CTAs.  Eight 16-bit elements per thread take 64 registers (1024 threads per SM), eight others up to 96 (640), sixteen up to 128 (512), thirty-two 234 (256);
 // what counts is the bytes on their way, 32 to 64 KB per SM in each case.  As many CTAs as are resident at once.
 BwdShape bwd_shape(long long rows, int dim, bool packed16) {
   if (dim > LN_LONGEST) return {1024, 1, (int)std::min<long long>(rows, kNumSMs)};

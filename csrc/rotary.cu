@@ -180,7 +180,7 @@ void launch_rotary(RotaryArgs& p, bool interleaved, cudaStream_t stream) {
 }
 
 // Elements per access: as many as 16 bytes hold, or the largest half of that which divides the rotated half, the head and all distances and addresses
-// (2 x 4096 x 40 heads of 80, 20 rotated: 97 us by single elements, 34 by pairs).
+// (2 x 4096 x 40 heads of 80, 20 rotated: 97 us by single elements, 36 by pairs).
 template <typename T>
 void by_width(RotaryArgs& p, int fit, bool interleaved, cudaStream_t stream) {
   const int half = (int)p.half.d;

@@ -107,7 +107,7 @@ std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& po
 
 // ---- vocabulary loss ---------------------------------------------------------------------------------------------------------------
 struct VocabLossBackward : public Node {
-  SavedVariable hidden, weight, target;      // hidden and weight in bf16, as the products take them
+  SavedVariable hidden, weight, target;      // [rows, h], [vocabulary, h] in bf16 and [rows], as the products take them
   Tensor lse2, count, err, parameter;        // parameter: of the trainer's arena, its gradient buffer is added to
   std::vector<int64_t> shape;                // of the hidden states as they were given
   int64_t reduction, workspace;
@@ -130,7 +130,7 @@ struct VocabLossBackward : public Node {
       const Tensor& own = parameter.grad();
       if (own.defined() && own.scalar_type() == at::kFloat && own.is_contiguous() && own.size(1) % 4 == 0 && (reinterpret_cast<uintptr_t>(own.data_ptr()) & 15) == 0) buffer = own;
     }
-    auto out = vocab_loss_bwd(g, h.dim() == 2 ? h : h.view({-1, w.size(1)}), w, t.dim() == 1 ? t : t.view({-1}), lse2, count, reduction, task_should_compute_output(0), fp32_dh, want_dw, fp32_dw, buffer, workspace, err);
+    auto out = vocab_loss_bwd(g, h, w, t, lse2, count, reduction, task_should_compute_output(0), fp32_dh, want_dw, fp32_dw, buffer, workspace, err);
     return {out.first.defined() && shape.size() != 2 ? out.first.view(shape) : out.first, out.second};
   }
 };
@@ -144,23 +144,24 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weig
     TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat, "vocabulary_cross_entropy: bf16 or fp32 hidden states and weight required");
   TORCH_CHECK_VALUE(hidden.is_cuda() && weight.device() == hidden.device() && target.device() == hidden.device(), "vocabulary_cross_entropy: hidden, weight and target on one device required");
   const bool grad = at::GradMode::is_enabled() && (wants_grad(hidden) || wants_grad(weight));
-  Tensor h16, t, loss, lse2, count;
+  Tensor h, w, t, loss, lse2, count;
   {
     const at::NoGradGuard none;
-    // kept as they were given where nothing has to be converted or copied: a change before the backward is then noticed
-    h16 = hidden.scalar_type() == at::kBFloat16 ? hidden : hidden.to(at::kBFloat16);
-    t = target.is_contiguous() ? target : target.contiguous();
-    const Tensor h2 = h16.dim() == 2 ? h16 : h16.reshape({-1, h16.size(-1)});
-    if (h16.dim() != 2 && !h16.is_contiguous()) h16 = h2;
-    auto out = vocab_loss_fwd(h2, weight16, t.dim() == 1 ? t : t.view({-1}), target.sizes(), reduction, err);
+    // Views of what was given where nothing has to be converted or copied: a change before the backward is then noticed.  Copies into padded rows are kept for it.
+    h = hidden.scalar_type() == at::kBFloat16 ? hidden : hidden.to(at::kBFloat16);
+    h = vocab_rows(h.dim() == 2 ? h : h.reshape({-1, h.size(-1)}));
+    // a bf16 copy of the weight that was made in inference mode cannot be saved
+    w = vocab_rows(grad && weight16.is_inference() ? weight.detach().to(at::kBFloat16) : weight16);
+    t = target.dim() == 1 ? target : target.reshape({-1});
+    if (!t.is_contiguous()) t = t.contiguous();
+    auto out = vocab_loss_fwd(h, w, t, target.sizes(), reduction, err);
     loss = out[0]; lse2 = out[1]; count = out[2];
   }
   if (grad) {
     auto node = std::shared_ptr<VocabLossBackward>(new VocabLossBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(hidden, weight));
-    node->hidden = SavedVariable(h16, false);
-    // a copy that was made in inference mode cannot be saved
-    node->weight = SavedVariable(weight16.is_inference() ? weight.detach().to(at::kBFloat16) : weight16, false);
+    node->hidden = SavedVariable(h, false);
+    node->weight = SavedVariable(w, false);
     node->target = SavedVariable(t, false);
     node->lse2 = lse2; node->count = count; node->err = err;
     if (managed) node->parameter = weight;

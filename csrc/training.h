@@ -26,7 +26,9 @@ std::pair<at::Tensor, at::Tensor> rotary_apply(const at::Tensor& q, const at::Te
 
 at::Tensor clip_grad_norm(at::TensorList grads, at::TensorList outs, double max_norm, bool scale);
 
-// hidden [rows, h], weight [vocabulary, h] bf16; reduction 0 none, 1 sum, 2 mean over the rows that count.
+// A bf16 matrix as TMA reads it: itself, or a copy in padded rows where its rows are not contiguous, on 16 bytes and a multiple of that apart.
+at::Tensor vocab_rows(const at::Tensor& t);
+// hidden [rows, h], weight [vocabulary, h] bf16, both as vocab_rows gives them; reduction 0 none, 1 sum, 2 mean over the rows that count.
 // `shape`: of the losses without a reduction.  Returns {loss (that shape, or 0-dim), log2 of the rows' sums [rows], number of rows that count (undefined without a reduction)}.
 std::array<at::Tensor, 3> vocab_loss_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, at::IntArrayRef shape, int64_t reduction,
                                          const at::Tensor& err);
