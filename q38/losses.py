@@ -37,7 +37,7 @@ def vocabulary_cross_entropy(weight, hidden, target, reduction="mean"):
     target's shape, 0 where a row does not count).
 
     On a GPU the scores exist as one piece's bf16 gradients at most; scores, sums and losses are fp32, and results have the same bits in every
-    run.  Where `linear_cross_entropy` keeps bf16 scores of all rows for the backward (vocabularies up to 16384), this forms them again: a quarter more
+    run.  Where `linear_cross_entropy` keeps bf16 scores of all rows for the backward (vocabularies up to 16384), this forms them again: a third more
     products for memory that does not grow with the vocabulary."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"vocabulary_cross_entropy: reduction must be mean, sum or none, got {reduction!r}")

@@ -109,7 +109,7 @@ def rotary(q, k, positions, frequencies, magnitude=1.0, interleaved=False):
         return q2.squeeze(0), None if k2 is None else k2.squeeze(0)
     if q.is_cuda:                                # checked there
         out = load().rotary(q, k, positions, frequencies, magnitude, interleaved)
-        return out if k is not None else (out[0], None)
+        return (out[0], out[1]) if k is not None else (out[0], None)
     _require(q.dim() == 4 and q.dtype in FLOATS, "rotary: fp32, bf16 or fp16 queries [batch, seq, heads, dim] required")
     B, S, _, D = q.shape
     if k is not None:

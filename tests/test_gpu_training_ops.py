@@ -67,7 +67,7 @@ def check_norm(x, w, b, dy, eps=1e-5, out_dtype=None):
 # widths: one element, a part of a warp, each kind of row (a warp with 8, 16 and 32 elements per thread; groups; 16 per thread; sums in shared memory; longer
 # than registers hold) at its ends, odd ones between; rows: none of a group's, one more than a CTA's, several rounds of the grid
 NORM_SHAPES = [(1, 1), (3, 7), (1, 64), (33, 256), (9, 257), (2500, 96), (17, 512), (5, 513), (6000, 520), (130, 1024), (64, 1025), (5, 2305), (700, 2048), (9, 4096), (7, 4097),
-               (3, 8192), (5, 8193), (2, 16384), (301, 8200), (2, 16385), (3, 20001)]
+               (3, 8192), (5, 8193), (2, 16384), (301, 8200), (2, 16385), (3, 20001), (100_003, 8), (70_000, 5)]
 
 
 @pytest.mark.parametrize("rows,dim", NORM_SHAPES)
@@ -213,7 +213,7 @@ def check_rotary(q, k, pos, f, m, interleaved):
 # batch, length, heads of queries and keys, head size, rotated part: the flagship's, one of everything, whole heads, odd pairs, a part that no vector fits,
 # heads of many units (one token per CTA), nothing rotated, more tokens than one round of the grid
 ROTARY_SHAPES = [(2, 65, 22, 2, 64, 16), (1, 1, 1, 1, 2, 2), (1, 7, 3, 1, 128, 128), (2, 5, 4, 2, 80, 20), (1, 9, 2, 2, 33, 6), (1, 3, 64, 8, 256, 256), (2, 4, 3, 1, 64, 0),
-                 (3, 1500, 4, 4, 32, 32), (1, 2, 5, 0, 48, 24), (16, 1, 22, 2, 64, 16), (1, 6, 300, 300, 72, 40)]
+                 (3, 1500, 4, 4, 32, 32), (1, 2, 5, 0, 48, 24), (16, 1, 22, 2, 64, 16), (1, 6, 300, 300, 72, 40), (1, 200_003, 1, 1, 8, 4)]
 
 
 @pytest.mark.parametrize("shape", ROTARY_SHAPES)
@@ -449,3 +449,35 @@ def test_operators_in_two_threads():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert all(torch.equal(a, b) for a, b in zip(results[0], results[1]))
+
+
+# ---- more elements than 32 bits count ---------------------------------------------------------------------------------------------------
+def test_layer_norm_of_more_than_2_31_elements():
+    rows, dim = 2_100_000, 1032
+    x = torch.randn(4096, dim, device="cuda").to(BF16).repeat(rows // 4096 + 1, 1)[:rows].requires_grad_()
+    w = torch.randn(dim, device="cuda")
+    y = ops.layer_norm(x, w)
+    dx, = torch.autograd.grad(y, x, y.detach())
+    tail = x.detach()[-7:].clone().requires_grad_()
+    y7 = ops.layer_norm(tail, w)
+    assert torch.equal(y[-7:], y7) and torch.equal(dx[-7:], torch.autograd.grad(y7, tail, y7.detach())[0])
+
+
+def test_rotary_of_more_than_2_31_elements():
+    f = ops.rotary_frequencies(256, device="cuda")[0]
+    tokens = 2_200_000
+    q = torch.randn(1, 4096, 4, 256, device="cuda").to(BF16).repeat(1, tokens // 4096 + 1, 1, 1)[:, :tokens]
+    pos = torch.arange(tokens, device="cuda")
+    out = ops.rotary(q, None, pos, f)[0]
+    assert torch.equal(out[:, -9:], ops.rotary(q[:, -9:], None, pos[-9:], f)[0])
+
+
+def test_clip_of_more_than_2_31_elements():
+    n = 2 ** 31 + 77
+    g = torch.full((n,), 2.0 ** -10, device="cuda", dtype=BF16)
+    g[-3:] = 1.0
+    norm = ops.clip_grad_norm([g], 1.0)
+    want = math.sqrt((n - 3) * 2.0 ** -20 + 3)
+    assert abs(norm.item() / want - 1) <= 2 * U
+    scaled = torch.tensor([2.0 ** -10 / want, 1 / want]).to(BF16).tolist()
+    assert g[0].item() == g[n // 2].item() == g[-4].item() == scaled[0] and g[-3:].tolist() == [scaled[1]] * 3

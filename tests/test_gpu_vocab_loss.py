@@ -87,7 +87,7 @@ def check(h, w, target, reduction="mean", up=None):
 
 # one of everything; a vocabulary within a chunk; hidden sizes that no TMA row fits; the ends of tiles in rows and columns; the presets' vocabulary; the larger tokenizers'
 SHAPES = [(1, 1, 8), (1, 5, 7), (2, 31, 1), (3, 300, 64), (37, 10112, 448), (128, 256, 64), (129, 257, 72), (257, 1000, 65), (1000, 5003, 200), (1500, 30080, 128), (5, 50048, 64),
-          (4100, 2049, 96), (20000, 65, 40)]
+          (4100, 2049, 96), (20000, 65, 40), (3, 200_003, 40)]
 
 
 @pytest.mark.parametrize("rows,vocab_size,hidden", SHAPES)
@@ -290,3 +290,15 @@ def test_changes_before_the_backward_are_noticed():
             (mid, mid_w, target)[what].add_(1)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             loss.backward()
+
+
+def test_more_scores_than_2_31():
+    h, w, target = inputs(70_000, 40_000, 16, seed=17)
+    leaf = h.requires_grad_()
+    loss = vocabulary_cross_entropy(w, leaf, target, "none")
+    up = torch.rand_like(loss)
+    dh, = torch.autograd.grad(loss, leaf, up)
+    tail = slice(-70, None)
+    (losses, _, want, _), (loss_off, dh_off, _) = formula(h.detach()[tail], w, target[tail], up[tail])
+    within(loss[tail], losses, loss_off, "losses")
+    within(dh[tail], want, dh_off, "dh")
