@@ -34,6 +34,10 @@ template <int CAP> struct ClipList {
 
 constexpr int CLIP_THREADS = 512;
 
+// The build flushes denormal fp32 values; a factor of one is to leave every value as it is, and small squares are to count
+__device__ __forceinline__ float clip_times(float a, float b) { float r; asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ double clip_wide(float a) { double r; asm("cvt.f64.f32 %0, %1;" : "=d"(r) : "f"(a)); return r; }
+
 template <int CAP>
 __device__ __forceinline__ int clip_find(const ClipList<CAP>& l, int piece) {
   int lo = 0, hi = l.count - 1;    // the last tensor whose first piece is not behind `piece`
@@ -53,7 +57,7 @@ __device__ __noinline__ double clip_apart(uint32_t w0, uint32_t w1) {
   unpack(p, f);
   double s = 0.0;
 #pragma unroll 1
-  for (int e = 0; e < 4; ++e) { const double d = (double)(e == 0 ? f[0] : e == 1 ? f[1] : e == 2 ? f[2] : f[3]); s += d * d; }
+  for (int e = 0; e < 4; ++e) { const double d = clip_wide(e == 0 ? f[0] : e == 1 ? f[1] : e == 2 ? f[2] : f[3]); s += d * d; }
   return s;
 }
 
@@ -89,12 +93,12 @@ __device__ __forceinline__ void clip_squares(const T* in, int n, double (&acc)[2
         float f[VEC];
         unpack(v[j], f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) { const double d = (double)f[e]; acc[(VEC == 1 ? j : e) & 1] += d * d; }
+        for (int e = 0; e < VEC; ++e) { const double d = clip_wide(f[e]); acc[(VEC == 1 ? j : e) & 1] += d * d; }
       }
     }
   }
 #pragma unroll 1
-  for (int i = packs * VEC + threadIdx.x; i < n; i += CLIP_THREADS) { const double d = (double)to_float(in[i]); acc[0] += d * d; }
+  for (int i = packs * VEC + threadIdx.x; i < n; i += CLIP_THREADS) { const double d = clip_wide(to_float(in[i])); acc[0] += d * d; }
 }
 
 template <typename T, int VEC>
@@ -113,12 +117,12 @@ __device__ __forceinline__ void clip_scale(const T* in, T* out, int n, float fac
         float f[VEC];
         unpack(v[j], f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] *= factor;
+        for (int e = 0; e < VEC; ++e) f[e] = clip_times(f[e], factor);
         store_pack<T, VEC>(out + (base + j * CLIP_THREADS) * VEC, pack<T, VEC>(f));
       }
   }
 #pragma unroll 1
-  for (int i = packs * VEC + threadIdx.x; i < n; i += CLIP_THREADS) out[i] = from_float<T>(to_float(in[i]) * factor);
+  for (int i = packs * VEC + threadIdx.x; i < n; i += CLIP_THREADS) out[i] = from_float<T>(clip_times(to_float(in[i]), factor));
 }
 
 // Calls f(typed pointer, elements per 16 bytes) of a tensor

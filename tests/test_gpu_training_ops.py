@@ -340,6 +340,14 @@ def test_clip_squares_neither_overflow_nor_vanish(value, count):
         assert norm.isinf()
 
 
+def test_clip_keeps_denormal_values():
+    tiny = torch.tensor([1e-40, -3e-39, 1.0, 0.0], device="cuda").repeat(700)
+    grads = [tiny, tiny.to(BF16), tiny[1:]]
+    out = [torch.zeros_like(g) for g in grads]
+    ops.clip_grad_norm(grads, 1e9, out=out)
+    assert all(torch.equal(o.view(torch.int32 if o.dtype == FP32 else torch.int16), g.view(torch.int32 if g.dtype == FP32 else torch.int16)) for o, g in zip(out, grads))
+
+
 def test_clip_values_that_are_not_finite():
     for bad in (float("nan"), float("inf")):
         g, h = torch.ones(100, device="cuda"), torch.ones(5000, device="cuda", dtype=BF16)

@@ -119,6 +119,7 @@ def test_strides_and_leading_dimensions():
     wide, tall = rand(60, 200), rand(1001, 129)
     check(wide[:, 8:72], (0.2 * tall)[:500, 1:65], target)           # rows apart; off 16 bytes
     check(rand(64, 60).t(), (0.2 * rand(64, 500)).t(), target)       # columns apart
+    check(wide[:, :65], (0.2 * rand(500, 136))[:, :65], target)      # rows that TMA takes, an odd number of their columns
     check(rand(1, 64).expand(60, 64), 0.2 * rand(500, 64), target)
     h, w = rand(3, 20, 64), 0.2 * rand(500, 64)
     got = vocabulary_cross_entropy(w, h, target.view(3, 20), "none")
