@@ -68,24 +68,32 @@ template <int VEC> __device__ __forceinline__ void param_pairs(const float* p, i
 __device__ __forceinline__ uint64_t twice(float a) { return pair2(a, a); }
 __device__ __forceinline__ float both(uint64_t a) { const float2 f = unpair(a); return f.x + f.y; }
 
-// Sums of a and b over a group of G threads.  `scratch` belongs to the group (2 x 32 pairs, used in turn, so that one barrier per sum is enough:
+// Sums of N values over a group of G threads.  `scratch` belongs to the group (two halves of 32 per value, used in turn, so that one barrier per sum is enough:
 // a thread writes a half again only after a barrier that all reach after they have read it).
-template <bool WARP>
-__device__ __forceinline__ float2 ln_group_sum(float a, float b, float2* scratch, int& turn, int G, int group) {
+template <bool WARP, int N>
+__device__ __forceinline__ void ln_group_sum(float (&v)[N], float* scratch, int& turn, int G, int group) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+  for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
   if constexpr (!WARP) {
     const int t = threadIdx.x - group * G, warps = G >> 5;
-    float2* s = scratch + turn * 32;
+    float* s = scratch + turn * 32 * N;
     turn ^= 1;
-    if ((t & 31) == 0) s[t >> 5] = make_float2(a, b);
-    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(G) : "memory");
-    const float2 v = (t & 31) < warps ? s[t & 31] : make_float2(0.f, 0.f);
-    a = v.x; b = v.y;
+    if ((t & 31) == 0) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) { a += __shfl_xor_sync(0xffffffffu, a, o); b += __shfl_xor_sync(0xffffffffu, b, o); }
+      for (int i = 0; i < N; ++i) s[i * 32 + (t >> 5)] = v[i];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(G) : "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (t & 31) < warps ? s[i * 32 + (t & 31)] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
   }
-  return make_float2(a, b);
 }
 
 // A thread's part of the weight and the bias: read once for all its rows where registers allow.  Read for every row they cost more of L1 than the row itself:
@@ -122,7 +130,7 @@ template <int VEC, int N, bool KEPT> struct LnParams {
 template <typename InT, typename OutT, int VEC, int E, bool WARP>
 __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E == 16 ? 3 : 2) layer_norm_fwd_kernel(LnArgs p) {
   grid_wait();
-  __shared__ float2 scratch[WARP ? 1 : 8][64];
+  __shared__ float scratch[WARP ? 1 : 8][64];
   constexpr int N = E / VEC;
   constexpr bool KEPT = WARP || E == 8;                          // otherwise 1024 threads leave no registers for it
   constexpr bool AHEAD = E <= 16 || (VEC > 1 && sizeof(InT) == 2);
@@ -150,7 +158,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E 
       for (int c = 0; c < N; ++c) v[c] = next[c];
       fetch(row + stride, next);
     } else fetch(row, v);
-    float mu, ss = 0.f;
+    float one[1], mu, ss = 0.f;
     if constexpr (VEC > 1) {
       uint64_t acc = 0;
 #pragma unroll
@@ -166,7 +174,9 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E 
 #pragma unroll
       for (int c = 0; c < E; ++c) { float f[1]; unpack(v[c], f); mu += f[0]; }
     }
-    mu = ln_group_sum<WARP>(mu, 0.f, scratch[WARP ? 0 : group], turn, G, group).x * inv;
+    one[0] = mu;
+    ln_group_sum<WARP>(one, scratch[WARP ? 0 : group], turn, G, group);
+    mu = one[0] * inv;
 #pragma unroll
     for (int c = 0; c < N; ++c) forget(v[c]);
     if constexpr (VEC > 1) {
@@ -183,7 +193,9 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E 
 #pragma unroll
       for (int c = 0; c < E; ++c) { float f[1]; unpack(v[c], f); const float d = c * G + t < p.dim ? f[0] - mu : 0.f; ss += d * d; }
     }
-    const float r = rsqrtf(ln_group_sum<WARP>(ss, 0.f, scratch[WARP ? 0 : group], turn, G, group).x * inv + p.eps);
+    one[0] = ss;
+    ln_group_sum<WARP>(one, scratch[WARP ? 0 : group], turn, G, group);
+    const float r = rsqrtf(one[0] * inv + p.eps);
     if (t == 0 && p.mean != nullptr) { p.mean[row] = mu; p.rstd[row] = r; }
 #pragma unroll
     for (int c = 0; c < N; ++c) forget(v[c]);
@@ -221,7 +233,7 @@ template <typename InT, typename OutT, int VEC, int E, bool WARP, bool ACC_SMEM>
 __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VEC != 8 ? 640 : 512, E == 8 && VEC == 8 ? 2 : 1) layer_norm_bwd_kernel(LnArgs p) {
   grid_wait();
   extern __shared__ float sums[];                                // [groups][2][dim]
-  __shared__ float2 scratch[16][64];
+  __shared__ float scratch[WARP ? 1 : 16][128];
   constexpr int N = E / VEC;
   const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
   const bool wanted = p.partial != nullptr;
@@ -306,11 +318,12 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VE
         }
       }
     }
-    const float2 s = ln_group_sum<WARP>(s1, s2, scratch[WARP ? 0 : group], turn, G, group);
+    float s[2] = {s1, s2};
+    ln_group_sum<WARP>(s, scratch[WARP ? 0 : group], turn, G, group);
 #pragma unroll
     for (int c = 0; c < N; ++c) { forget(x[c]); forget(d[c]); }
     if (p.out != nullptr) {
-      const float k0 = s.x * inv * r, k1 = s.y * inv * r * r;    // dx = r g - k0 - (x - mu) k1
+      const float k0 = s[0] * inv * r, k1 = s[1] * inv * r * r;    // dx = r g - k0 - (x - mu) k1
       InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
 #pragma unroll
       for (int c = 0; c < N; ++c) {                              // from the packed row again: the values themselves would take twice its registers
