@@ -108,13 +108,13 @@ template <int VEC, int N, bool KEPT> struct LnParams {
     if constexpr (VEC > 1) param_pairs<VEC>(p, at, out, none); else ln_param<1>(p, at, out, none);
   }
   // zeros behind a row's end
-  __device__ __forceinline__ LnParams(const float* p_, float none_, int G, int t, int dim) : p(p_), none(none_) {
+  __device__ __forceinline__ LnParams(const float* p_, float none_, int first, int dim) : p(p_), none(none_) {
     if constexpr (KEPT) {
 #pragma unroll
       for (int c = 0; c < N; ++c) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) v[c][i] = 0;
-        if ((c * G + t) * VEC < dim) read((c * G + t) * VEC, v[c]);
+        if (first + c * 32 * VEC < dim) read(first + c * 32 * VEC, v[c]);
       }
     }
   }
@@ -135,16 +135,17 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E 
   constexpr bool KEPT = WARP || E == 8;                          // otherwise 1024 threads leave no registers for it
   constexpr bool AHEAD = E <= 16 || (VEC > 1 && sizeof(InT) == 2);
   const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
+  const int first = (t >> 5) * 32 * E + (t & 31) * VEC;          // a warp's columns lie side by side, a thread's at fixed distances: accesses need no arithmetic
   const float inv = 1.f / p.dim;
   const long long stride = (long long)gridDim.x * p.groups;
-  const LnParams<VEC, N, KEPT> weight(p.w, 1.f, G, t, p.dim), bias(p.b, 0.f, G, t, p.dim);
+  const LnParams<VEC, N, KEPT> weight(p.w, 1.f, first, p.dim), bias(p.b, 0.f, first, p.dim);
   Pack<InT, VEC> v[N] = {}, next[AHEAD ? N : 1] = {};            // rows as they came: half the registers for 16-bit types
   auto fetch = [&](long long at_row, auto& to) {
     if (at_row >= p.rows) return;
     const InT* x = reinterpret_cast<const InT*>(p.x) + at_row * p.ldx;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int at = (c * G + t) * VEC;
+      const int at = first + c * 32 * VEC;
       if (at < p.dim) to[c] = load_pack<InT, VEC>(x + at);
     }
   };
@@ -187,11 +188,11 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E 
         pairs_of(v[c], f);
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) { const uint64_t d = add2(f[i], minus); acc = fma2(d, d, acc); }
-        ss += (c * G + t) * VEC < p.dim ? both(acc) : 0.f;
+        ss += first + c * 32 * VEC < p.dim ? both(acc) : 0.f;
       }
     } else {
 #pragma unroll
-      for (int c = 0; c < E; ++c) { float f[1]; unpack(v[c], f); const float d = c * G + t < p.dim ? f[0] - mu : 0.f; ss += d * d; }
+      for (int c = 0; c < E; ++c) { float f[1]; unpack(v[c], f); const float d = first + c * 32 < p.dim ? f[0] - mu : 0.f; ss += d * d; }
     }
     one[0] = ss;
     ln_group_sum<WARP>(one, scratch[WARP ? 0 : group], turn, G, group);
@@ -202,7 +203,7 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E 
     OutT* y = reinterpret_cast<OutT*>(p.out) + row * p.dim;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int at = (c * G + t) * VEC;
+      const int at = first + c * 32 * VEC;
       if (at < p.dim) {
         float o[VEC];
         if constexpr (VEC > 1) {
@@ -230,15 +231,16 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024, !WARP ? 1 : E == 8 ? 4 : E 
 
 // ACC: where the weight sums of a thread's columns live (registers, or shared memory for rows so long that registers would spill; each cell has one owner).
 template <typename InT, typename OutT, int VEC, int E, bool WARP, bool ACC_SMEM>
-__global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VEC != 8 ? 640 : 512, E == 8 && VEC == 8 ? 2 : 1) layer_norm_bwd_kernel(LnArgs p) {
+__global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 ? (VEC == 8 ? 384 : 640) : 512, E == 8 && VEC == 8 ? 2 : 1) layer_norm_bwd_kernel(LnArgs p) {
   grid_wait();
   extern __shared__ float sums[];                                // [groups][2][dim]
   __shared__ float scratch[WARP ? 1 : 16][128];
   constexpr int N = E / VEC;
   const int G = WARP ? 32 : blockDim.x / p.groups, group = threadIdx.x / G, t = threadIdx.x - group * G;
+  const int first = (t >> 5) * 32 * E + (t & 31) * VEC;          // a warp's columns lie side by side, a thread's at fixed distances: accesses need no arithmetic
   const bool wanted = p.partial != nullptr;
   constexpr bool KEPT = !ACC_SMEM && (E != 16 || (VEC > 1 && sizeof(InT) == 2));
-  const LnParams<VEC, N, KEPT> weight(p.w, 1.f, G, t, p.dim);
+  const LnParams<VEC, N, KEPT> weight(p.w, 1.f, first, p.dim);
   const float inv = 1.f / p.dim;
   using Acc = std::conditional_t<(VEC > 1), uint64_t, float>;    // pairs of columns, or single ones
   constexpr int ACCS = ACC_SMEM ? 1 : VEC > 1 ? E / 2 : E;
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VE
     nmu = p.mean[at_row]; nr = p.rstd[at_row];
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int at = (c * G + t) * VEC;
+      const int at = first + c * 32 * VEC;
       if (at < p.dim) {
         nx[c] = load_pack<InT, VEC>(px + at);
         nd[c] = load_pack<OutT, VEC>(pd + at);
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VE
       uint64_t t1 = 0, t2 = 0;
 #pragma unroll
       for (int c = 0; c < N; ++c) {
-        const int at = (c * G + t) * VEC;
+        const int at = first + c * 32 * VEC;
         uint64_t xv[VEC / 2], dv[VEC / 2], w[VEC / 2] = {};
         pairs_of(x[c], xv);
         pairs_of(d[c], dv);
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VE
     } else {
 #pragma unroll
       for (int c = 0; c < N; ++c) {
-        const int at = (c * G + t) * VEC;
+        const int at = first + c * 32 * VEC;
         if (at < p.dim) {
           float xv[VEC], dv[VEC], w[VEC];
           unpack(x[c], xv);
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VE
       InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
 #pragma unroll
       for (int c = 0; c < N; ++c) {                              // from the packed row again: the values themselves would take twice its registers
-        const int at = (c * G + t) * VEC;
+        const int at = first + c * 32 * VEC;
         if (at < p.dim) {
           float o[VEC];
           if constexpr (VEC > 1) {
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 && VE
     float* to = p.groups == 1 ? mine : sums + (long long)group * 2 * p.dim;
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      const int at = (c * G + t) * VEC;
+      const int at = first + c * 32 * VEC;
       if (at < p.dim) {
         if constexpr (VEC > 1) {
 #pragma unroll
@@ -505,14 +507,14 @@ struct BwdShape { int G, groups, ctas; };
 // Elements per thread: eight, or more.  The sums over a group cost some sixty instructions per thread and row, so packed rows, which have the registers, take sixteen or thirty-two.
 bool eight_each(int dim, bool packed16) { return dim <= 256 || (!packed16 && dim > 512 && dim <= 4096); }
 
-// Threads per row, rows per CTA and CTAs.  Eight 16-bit elements per thread take 64 registers (1024 threads per SM), eight others up to 96 (640), sixteen up to 128 (512), thirty-two 234 (256);
+// Threads per row, rows per CTA and CTAs.  Eight 16-bit elements per thread take 80 registers (768 threads per SM), eight others up to 96 (640), sixteen up to 128 (512), thirty-two 234 (256);
 // what counts is the bytes on their way, 32 to 64 KB per SM in each case.  As many CTAs as are resident at once.
 BwdShape bwd_shape(long long rows, int dim, bool packed16) {
   if (dim > LN_LONGEST) return {1024, 1, (int)std::min<long long>(rows, kNumSMs)};
   BwdShape s;
   const bool eight = eight_each(dim, packed16);
   const bool warp32 = packed16 && dim > 512 && dim <= 1024;      // thirty-two per thread: a warp holds the row, no barrier
-  const int threads = warp32 ? 256 : eight && !packed16 ? 320 : 512, resident = warp32 ? 256 : eight ? (packed16 ? 1024 : 640) : 512;
+  const int threads = warp32 ? 256 : eight ? (packed16 ? 384 : 320) : 512, resident = warp32 ? 256 : eight ? (packed16 ? 768 : 640) : 512;
   s.G = dim <= 512 || warp32 ? 32 : group_of(dim, eight ? 8 : 16);
   s.groups = std::max(1, threads / s.G);
   s.ctas = (int)std::min<long long>((rows + s.groups - 1) / s.groups, std::max(1, resident / (s.G * s.groups)) * kNumSMs);
