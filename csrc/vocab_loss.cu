@@ -12,6 +12,8 @@
 // The kernel follows csrc/gemm_persistent.cu: one CTA per SM, warp 0 loads by TMA, one lane of warp 1 issues the MMAs into one of two accumulators, and eight
 // warps (two warpgroups on alternate 32-column chunks) read the other.  Tiles are walked with the rows fastest, in groups of rows whose hidden states
 // stay in L2: all SMs work on the same few columns of W, which so comes from memory once per group.
+// On a B200, each kernel alone: 8192 x 50048 x 1024 forward 513 us (1.64 PFLOP/s, level with cuBLAS), dz 629 us (1.33), dh and dW 608 and 582 us; 4096 x 10112 x 576
+// 38, 44, 43 and 48 us.  Bound by the tensor cores in the forward, by operand traffic (96 bytes per clock and SM, and the stores of dz) in the others.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
