@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 ? (VE
 #pragma unroll
     for (int c = 0; c < N; ++c) { forget(x[c]); forget(d[c]); }
     if (p.out != nullptr) {
-      const float k0 = s[0] * inv * r, k1 = s[1] * inv * r * r;    // dx = r g - k0 - (x - mu) k1
+      const float k0 = s[0] * inv * r, k1 = s[1] * inv * r;        // dx = r g - k0 - xhat k1 (r r could overflow where eps is zero)
       InT* dx = reinterpret_cast<InT*>(p.out) + row * p.dim;
 #pragma unroll
       for (int c = 0; c < N; ++c) {                              // from the packed row again: the values themselves would take twice its registers
@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 ? (VE
             weight.get(c, at, w);
 #pragma unroll
             for (int i = 0; i < VEC / 2; ++i) {
-              const float2 f = unpair(fma2(dv[i], mul2(w[i], twice(r)), fma2(add2(xv[i], twice(-mu)), twice(-k1), twice(-k0))));
+              const uint64_t hat = mul2(add2(xv[i], twice(-mu)), twice(r));
+              const float2 f = unpair(fma2(dv[i], mul2(w[i], twice(r)), fma2(hat, twice(-k1), twice(-k0))));
               o[2 * i] = f.x; o[2 * i + 1] = f.y;
             }
           } else {
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 ? (VE
             unpack(x[c], o);
             unpack(d[c], dv);
             weight.get(c, at, w);
-            o[0] = dv[0] * (w[0] * r) - ((o[0] - mu) * k1 + k0);
+            o[0] = dv[0] * (w[0] * r) - ((o[0] - mu) * r * k1 + k0);
           }
           store_pack<InT, VEC>(dx + at, pack<InT, VEC>(o));
         }

@@ -117,6 +117,23 @@ def test_layer_norm_strides_and_offsets():
     within(g, want[1].sum(0, keepdim=True), 250 * U * size[1].sum(0, keepdim=True), "row")
 
 
+def test_layer_norm_of_tiny_values_without_eps():
+    """A spread of 1e-18: its inverse is finite in fp32, the square of that is not."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=gen)
+    for dim in (256, 777, 1500):
+        x, dy = 1e-18 * rand(6, dim), rand(6, dim)
+        leaf = x.requires_grad_()
+        y = ops.layer_norm(leaf, eps=0.0)
+        want, size = norm_formula(x.detach(), None, None, dy, 0.0)
+        # Squares under the smallest normal number, 2^-126, count as zero: the variance v (about 1e-36) loses at most that, so 1 / sqrt(v) is off by at most
+        # 0.51 * 2^-126 / v of itself (v (1 - a))^-1/2 = v^-1/2 (1 + a / 2 + ...), a < 0.02), and with it each of the up to three factors 1 / sqrt(v) in dx
+        lost = 0.51 * 2.0 ** -126 / x.detach().double().var(-1, unbiased=False, keepdim=True)
+        assert lost.max() < 0.01
+        within(y, want[0], (100 * U + lost) * size[0], "y")
+        within(torch.autograd.grad(y, leaf, dy)[0], want[1], (200 * U + 3.1 * lost) * size[1], "dx")
+
+
 def test_layer_norm_empty_and_not_finite():
     w = torch.ones(64, device="cuda", requires_grad=True)
     x = torch.zeros(0, 64, device="cuda", dtype=BF16, requires_grad=True)
