@@ -17,6 +17,7 @@
 #include "ptx.cuh"
 #include "host.h"
 #include "launch.cuh"
+#include "training.h"
 
 namespace q38 {
 
@@ -319,8 +320,7 @@ static void launch_p(const CUtensorMap& ta, const CUtensorMap& tb, const CUtenso
   const int grid = std::min(p.work_items, kNumSMs);
   Q38_TRACE("[gemm_p] launch grid=%d smem=%d bn=%d items=%d splits=%d kb=%d tma_out=%d fp32=%d acc=%d amn=%d bmn=%d\n", grid, smem, p.bn, p.work_items, p.splits,
             p.total_kb, (int)tma_out, (int)out_fp32, (int)accum, (int)A_MN, (int)B_MN);
-#define Q38_LAUNCH(OutT, ACC, TMAO) { auto k = gemm_persistent_kernel<A_MN, B_MN, OutT, ACC, TMAO, TF32>; static bool cfg = false; \
-    if (!cfg) { C10_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024)); cfg = true; } \
+#define Q38_LAUNCH(OutT, ACC, TMAO) { auto k = gemm_persistent_kernel<A_MN, B_MN, OutT, ACC, TMAO, TF32>; allow_shared_memory((const void*)k, 227 * 1024); \
     launch(k, grid, P_THREADS, smem, stream, ta, tb, tc, p); }
   if constexpr (TF32) {
     if (!out_fp32) { if (tma_out) Q38_LAUNCH(__nv_bfloat16, false, true) else Q38_LAUNCH(__nv_bfloat16, false, false) }
