@@ -150,8 +150,7 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weig
     // Views of what was given where nothing has to be converted or copied: a change before the backward is then noticed.  Copies into padded rows are kept for it.
     h = hidden.scalar_type() == at::kBFloat16 ? hidden : hidden.to(at::kBFloat16);
     h = vocab_rows(h.dim() == 2 ? h : h.reshape({-1, h.size(-1)}));
-    // a bf16 copy of the weight that was made in inference mode cannot be saved
-    w = vocab_rows(grad && weight16.is_inference() ? weight.detach().to(at::kBFloat16) : weight16);
+    w = vocab_rows(weight16);
     t = target.dim() == 1 ? target : target.reshape({-1});
     if (!t.is_contiguous()) t = t.contiguous();
     auto out = vocab_loss_fwd(h, w, t, target.sizes(), reduction, err);

@@ -31,7 +31,8 @@ def linear_cross_entropy(weight, hidden, target, reduction="mean"):
 def vocabulary_cross_entropy(weight, hidden, target, reduction="mean"):
     """Softmax cross entropy of ``hidden @ weight.T`` against ``target`` for vocabularies of any size, without keeping logits.
 
-    hidden: ``[..., h]`` bf16 or fp32 (rounded to bf16 for the products); weight: ``[vocabulary, h]`` bf16, or fp32 as a master weight; target: int64 of
+    hidden: ``[..., h]`` bf16 or fp32 (rounded to bf16 for the products); weight: ``[vocabulary, h]`` bf16, or fp32 as a master weight (rounded to bf16 by every
+    call, unless the trainer's arena keeps its bf16 form); target: int64 of
     hidden's leading shape, -100 where a row does not count (any other target outside the vocabulary counts as -100 and raises at
     `q38.ops.check_errors`).  ``reduction``: ``"mean"`` over the rows that count (0 where none does), ``"sum"``, or ``"none"`` (fp32 losses of
     target's shape, 0 where a row does not count).

@@ -1,0 +1,100 @@
+"""Calls of the operators around a training step in graphs, on several streams, in inference mode and under other transforms."""
+import pytest
+import torch
+
+from q38 import ops
+from q38.losses import vocabulary_cross_entropy
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def installed():
+    ops.install()
+    yield
+    ops.check_errors()
+
+
+# ---- vocabulary loss with an fp32 weight ---------------------------------------------------------------------------------------------
+def master(seed, rows=200, words=3000, width=64):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    h = torch.randn(rows, width, device="cuda", generator=gen).to(BF16)
+    w = torch.randn(words, width, device="cuda", generator=gen) * 0.3
+    return h.requires_grad_(), w.requires_grad_(), torch.randint(0, words, (rows,), device="cuda", generator=gen)
+
+
+def step(h, w, target):
+    loss = vocabulary_cross_entropy(w, h, target)
+    return (loss.detach(), *torch.autograd.grad(loss, [h, w]))
+
+
+def from_bf16(h, w, target):
+    """The same with a weight that is bf16 from the start."""
+    loss, dh, dw = step(h, w.detach().to(BF16).requires_grad_(), target)
+    return loss, dh, dw
+
+
+def same(got, want):
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(got[2].to(BF16), want[2])                       # the fp32 gradient, rounded as the other is
+
+
+@pytest.mark.parametrize("width", [64, 71])
+def test_master_weight_changes_between_replays(width):
+    h, w, target = master(0, width=width)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            step(h, w, target)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(h, w, target)
+    for change in (lambda: w.mul_(1.5), lambda: w.data.mul_(-0.5), lambda: w.data.copy_(master(1, width=width)[1])):
+        with torch.no_grad():
+            change()
+        graph.replay()
+        same(held, from_bf16(h, w, target))
+    step(h, w, target)
+    graph.replay()
+    same(held, from_bf16(h, w, target))
+
+
+def test_master_weight_on_a_second_stream():
+    """The first call's rounding waits behind a long kernel on its stream; the second call, on a stream of its own, must not depend on it."""
+    h, w, target = master(2)
+    want = step(h, w, target)
+    with torch.no_grad():
+        w.add_(0)                                                     # a version that no call has seen
+    torch.cuda.synchronize()
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(first):
+        torch.cuda._sleep(50_000_000)
+        one = step(h, w, target)
+    with torch.cuda.stream(second):
+        two = step(h, w, target)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for got in (one, two) for a, b in zip(got, want))
+
+
+def test_master_weight_changes_outside_the_version_counter():
+    h, w, target = master(3)
+    step(h, w, target)
+    w.data.mul_(2)
+    same(step(h, w, target), from_bf16(h, w, target))
+    w.data = w.data * 0.25
+    same(step(h, w, target), from_bf16(h, w, target))
+    assert not vars(w)
+
+
+def test_master_weight_made_in_inference_mode():
+    h, w, target = master(4)
+    with torch.inference_mode():
+        seen = w.detach().clone()
+        inside = vocabulary_cross_entropy(seen, h, target)
+    want = step(h, w, target)
+    loss = vocabulary_cross_entropy(seen, h, target)
+    assert torch.equal(inside, want[0]) and torch.equal(loss, want[0])
+    assert torch.equal(torch.autograd.grad(loss, h)[0], want[1])
