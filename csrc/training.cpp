@@ -1,6 +1,7 @@
 // Autograd nodes of the operators around a training step's products, and their registration.  The nodes are written out in C++: one in Python costs 10 to 20 us
 // per pass, torch's own wrapper for C++ functions half of that, and the kernels of a short sequence take 2 to 5.
 #include <ATen/ATen.h>
+#include <c10/core/DispatchKeySet.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -18,6 +19,17 @@ using torch::autograd::variable_list;
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
+
+// The entries are registered for every kind of tensor, and the kernels take addresses: a fake or wrapped tensor has a null one (a launch would fault), a batched or
+// transformed one none of its own.
+void own_memory(const char* name, const Tensor& t) {
+  constexpr c10::DispatchKeySet without{c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchGradWrapper,
+                                        c10::DispatchKey::ZeroTensor};
+  TORCH_CHECK_VALUE(!t.defined() || !t.key_set().has_any(without), name, ": a tensor with values in memory of its own is required, not one that is fake, wrapped, batched or transformed");
+}
+void own_memory(const char* name, const OptTensor& t) { if (t.has_value()) own_memory(name, *t); }
+void own_memory(const char* name, at::TensorList list) { for (const Tensor& t : list) own_memory(name, t); }
+
 void first_order_only(const char* name) { TORCH_CHECK(!at::GradMode::is_enabled(), name, ": a gradient of the gradient is not available"); }
 
 // ---- layer norm ---------------------------------------------------------------------------------------------------------------
@@ -34,6 +46,7 @@ struct LayerNormBackward : public Node {
     const std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("layer_norm");
     if (!grads[0].defined()) return variable_list(3);
+    own_memory("layer_norm", grads[0]);
     auto self = shared_from_this();
     const Tensor xs = x.unpack(self), ws = w.unpack(self);
     auto out = layer_norm_bwd(grads[0], xs, optional_of(ws), b, stats, task_should_compute_output(0), ws.defined() && task_should_compute_output(1),
@@ -43,6 +56,9 @@ struct LayerNormBackward : public Node {
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, c10::optional<at::ScalarType> out_type) {
+  own_memory("layer_norm", x);
+  own_memory("layer_norm", w);
+  own_memory("layer_norm", b);
   const Tensor wt = w.value_or(Tensor()), bt = b.value_or(Tensor());
   const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(wt) || wants_grad(bt));
   Tensor y, stats;
@@ -77,12 +93,15 @@ struct RotaryBackward : public Node {
     first_order_only("rotary");
     const Tensor dq = task_should_compute_output(0) ? grads[0] : Tensor(), dk = grads.size() > 1 && task_should_compute_output(1) ? grads[1] : Tensor();
     if (!dq.defined() && !dk.defined()) return variable_list(2);
+    own_memory("rotary", grads);
     auto out = rotary_apply(dq, dk, pos.unpack(), freq.unpack(), magnitude, interleaved, -1.0);
     return {out.first, out.second};
   }
 };
 
 std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& pos, const Tensor& frequencies, double magnitude, bool interleaved) {
+  for (const Tensor* t : {&q, &pos, &frequencies}) own_memory("rotary", *t);
+  own_memory("rotary", k);
   const Tensor freq = frequencies.is_contiguous() ? frequencies : frequencies.contiguous();
   rotary_check(q, k, pos, freq);
   const Tensor kt = k.value_or(Tensor());
@@ -122,6 +141,7 @@ struct VocabLossBackward : public Node {
     const std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("vocabulary_cross_entropy");
     if (!grads[0].defined()) return variable_list(2);
+    own_memory("vocabulary_cross_entropy", grads[0]);
     const Tensor h = hidden.unpack(), w = weight.unpack(), t = target.unpack();
     const Tensor g = grads[0].scalar_type() == at::kFloat && grads[0].is_contiguous() ? grads[0] : grads[0].to(at::kFloat).contiguous();
     const bool want_dw = task_should_compute_output(1);
@@ -137,6 +157,7 @@ struct VocabLossBackward : public Node {
 
 // hidden [..., h]; weight [vocabulary, h] and the same in bf16; target of hidden's leading shape.
 Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weight16, const Tensor& target, int64_t reduction, bool managed, int64_t workspace, const Tensor& err) {
+  for (const Tensor* t : {&hidden, &weight, &weight16, &target, &err}) own_memory("vocabulary_cross_entropy", *t);
   TORCH_CHECK_VALUE(weight.dim() == 2 && hidden.dim() >= 1 && hidden.size(-1) == weight.size(1) && weight.numel() > 0,
                     "vocabulary_cross_entropy: hidden [..., h] and weight [vocabulary, h] required");
   TORCH_CHECK_VALUE(target.sizes() == hidden.sizes().slice(0, hidden.dim() - 1) && target.scalar_type() == at::kLong, "vocabulary_cross_entropy: int64 targets of hidden's leading shape required");
@@ -172,6 +193,12 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weig
   return loss;
 }
 
+Tensor clip(const char* name, at::TensorList grads, at::TensorList outs, double max_norm, bool scale) {
+  own_memory(name, grads);
+  own_memory(name, outs);
+  return clip_grad_norm(grads, outs, max_norm, scale);
+}
+
 }  // namespace
 }  // namespace q38
 
@@ -179,7 +206,9 @@ TORCH_LIBRARY_FRAGMENT(q38, m) {
   m.def("layer_norm(Tensor x, Tensor? w, Tensor? b, float eps, ScalarType? out_dtype=None) -> Tensor", &q38::layer_norm);
   m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor frequencies, float magnitude, bool interleaved) -> Tensor[]", &q38::rotary);
   m.def("vocab_loss(Tensor hidden, Tensor weight, Tensor weight16, Tensor target, int reduction, bool managed, int workspace, Tensor(a!) err) -> Tensor", &q38::vocab_loss);
-  m.def("grad_norm(Tensor[] grads) -> Tensor", [](at::TensorList g) { return q38::clip_grad_norm(g, {}, 1.0, false); });
-  m.def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm) -> Tensor", [](at::TensorList g, double m) { return q38::clip_grad_norm(g, {}, m, true); });
-  m.def("clip_grad_norm_out(Tensor[] grads, Tensor(a!)[] out, float max_norm) -> Tensor", [](at::TensorList g, at::TensorList o, double m) { return q38::clip_grad_norm(g, o, m, true); });
+  m.def("grad_norm(Tensor[] grads) -> Tensor", [](at::TensorList g) { return q38::clip("grad_norm", g, {}, 1.0, false); });
+  m.def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm) -> Tensor", [](at::TensorList g, double m) { return q38::clip("clip_grad_norm", g, {}, m, true); });
+  m.def("clip_grad_norm_out(Tensor[] grads, Tensor(a!)[] out, float max_norm) -> Tensor",
+        [](at::TensorList g, at::TensorList o, double m) { return q38::clip("clip_grad_norm", g, o, m, true); });
+  m.def("own_memory(Tensor[] tensors, str name) -> ()", [](at::TensorList t, c10::string_view name) { q38::own_memory(std::string(name).c_str(), t); });
 }

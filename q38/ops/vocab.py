@@ -1,7 +1,7 @@
 """Cross entropy of a vocabulary projection in pieces of the vocabulary (`csrc/vocab_loss.cu`), behind `q38.losses.vocabulary_cross_entropy`."""
 import torch
 
-from . import error_flag, load
+from . import _error_flags, error_flag, load
 
 # Bytes that the score gradients of one piece of the vocabulary may take.  A piece of 256 MB is written and read twice at the memory's rate while its three
 # products take several times as long; smaller pieces only add launches and passes over the hidden gradient's sums.
@@ -13,6 +13,9 @@ def vocabulary_loss(hidden, weight, target, reduction):
     """hidden [..., h], weight [vocabulary, h], target [...] on one GPU; `reduction` a key of REDUCTIONS.  A parameter of the trainer's arena (it carries its bf16
     shadow) has its gradient added to its buffer in place, any other gets it returned.  An fp32 weight outside the arena is rounded by every call (50048 x 1024: 2 % of
     a training pass): a copy kept on the weight would be missing from a captured graph, unordered on a second stream and stale after a change through `.data`."""
+    lib = load()
+    if hidden.device.index not in _error_flags:
+        lib.own_memory([hidden, weight, target], "vocabulary_cross_entropy")   # before the device's error word is made and kept, which would be no memory either
     shadow = getattr(weight, "_q38_bf16", None)
     weight16 = shadow if shadow is not None else weight.detach().to(torch.bfloat16)
-    return load().vocab_loss(hidden, weight, weight16, target, REDUCTIONS[reduction], shadow is not None, PIECE_BYTES, error_flag(hidden.device))
+    return lib.vocab_loss(hidden, weight, weight16, target, REDUCTIONS[reduction], shadow is not None, PIECE_BYTES, error_flag(hidden.device))

@@ -98,3 +98,25 @@ def test_master_weight_made_in_inference_mode():
     loss = vocabulary_cross_entropy(seen, h, target)
     assert torch.equal(inside, want[0]) and torch.equal(loss, want[0])
     assert torch.equal(torch.autograd.grad(loss, h)[0], want[1])
+
+
+# ---- gradients that are no memory ------------------------------------------------------------------------------------------------------
+def outputs():
+    """A result of each differentiable operator and its leaf."""
+    x = torch.randn(6, 64, device="cuda", requires_grad=True)
+    q = torch.randn(1, 6, 2, 16, device="cuda", requires_grad=True)
+    h, w, target = master(5, 6, 100)
+    freq, _ = ops.rotary_frequencies(16, device="cuda")
+    return [(ops.layer_norm(x), x), (ops.rotary(q, None, torch.arange(6, device="cuda"), freq)[0], q), (vocabulary_cross_entropy(w, h, target, "none"), h)]
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_batched_gradients_are_refused(which):
+    y, leaf = outputs()[which]
+    with pytest.raises(ValueError, match="values in memory of its own"):
+        torch.autograd.grad(y, leaf, torch.ones(3, *y.shape, device="cuda"), is_grads_batched=True)
+
+
+def test_layer_norm_under_vmap():
+    x = torch.randn(3, 5, 64, device="cuda")
+    assert torch.equal(torch.func.vmap(ops.layer_norm)(x), ops.layer_norm(x))

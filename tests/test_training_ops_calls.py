@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from q38 import ops
 from q38.ops import vocab
 
 
@@ -10,6 +11,9 @@ class Native:
 
     def __init__(self):
         self.weights = []
+
+    def own_memory(self, tensors, name):
+        pass
 
     def vocab_loss(self, hidden, weight, weight16, target, reduction, managed, workspace, err):
         self.weights.append(weight16)
@@ -58,3 +62,92 @@ def test_a_bf16_weight_and_an_arena_shadow_go_in_as_they_are(native):
     managed._q38_bf16 = managed.to(torch.bfloat16)
     _call(managed)
     assert [w.data_ptr() for w in native.weights] == [weight.data_ptr(), managed._q38_bf16.data_ptr()]
+
+
+# ---- tensors that are no memory --------------------------------------------------------------------------------------------------------
+def _normal(x):
+    return ops.load().layer_norm(x, None, None, 1e-5)
+
+
+def _scaled(w):
+    return ops.load().layer_norm(torch.zeros(3, 8), w[0, 0], None, 1e-5)
+
+
+def _shifted(b):
+    return ops.load().layer_norm(torch.zeros(3, 8), None, b[0, 0], 1e-5)
+
+
+def _turned(q):
+    return ops.load().rotary(q[None], None, torch.zeros(4, dtype=torch.int64), torch.zeros(4, dtype=torch.float64), 1.0, False)
+
+
+def _turned_key(k):
+    return ops.load().rotary(torch.zeros(1, 4, 8, 8), k[None], torch.zeros(4, dtype=torch.int64), torch.zeros(4, dtype=torch.float64), 1.0, False)
+
+
+def _turned_at(pos):
+    return ops.load().rotary(torch.zeros(1, 4, 8, 8), None, pos.flatten()[:4].long(), torch.zeros(4, dtype=torch.float64), 1.0, False)
+
+
+def _turned_by(f):
+    return ops.load().rotary(torch.zeros(1, 4, 8, 8), None, torch.zeros(4, dtype=torch.int64), f.flatten()[:4].double(), 1.0, False)
+
+
+def _total(g):
+    return ops.load().grad_norm([torch.ones(3), g])
+
+
+def _clipped(g):
+    return ops.load().clip_grad_norm_([g], 1.0)
+
+
+def _clipped_into(o):
+    return ops.load().clip_grad_norm_out([torch.ones(4, 8, 8)], [o], 1.0)
+
+
+def _losses(h):
+    return vocab.vocabulary_loss(h, torch.zeros(11, 8), torch.zeros(h.shape[:-1], dtype=torch.int64), "none")
+
+
+def _losses_by(w):
+    return vocab.vocabulary_loss(torch.zeros(3, 8), w[0], torch.zeros(3, dtype=torch.int64), "mean")
+
+
+def _losses_of(t):
+    return vocab.vocabulary_loss(torch.zeros(3, 8), torch.zeros(11, 8), t.flatten()[:3].long(), "mean")
+
+
+class Wrapped(torch.Tensor):
+    """As sharded tensors are made: a device and sizes, and the values in another tensor."""
+
+    @staticmethod
+    def __new__(cls, inner, device):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=device)
+
+    def __init__(self, inner, device):
+        self.inner = inner
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        args = [a.inner if isinstance(a, cls) else a for a in args]
+        return cls(func(*args, **(kwargs or {})), "cuda")
+
+
+ENTRIES = [_normal, _scaled, _shifted, _turned, _turned_key, _turned_at, _turned_by, _total, _clipped, _clipped_into, _losses, _losses_by, _losses_of]
+
+
+@pytest.mark.parametrize("entry", ENTRIES)
+@pytest.mark.parametrize("kind", ["fake", "wrapped", "differentiated"])
+def test_tensors_without_memory_are_refused(entry, kind, monkeypatch):
+    """Their address is null, or not to be had.  They are refused before the error word is made, which would be one of them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    monkeypatch.setattr(ops, "_error_flags", flags := {})
+    with pytest.raises(ValueError, match="values in memory of its own"):
+        if kind == "fake":
+            with FakeTensorMode():
+                entry(torch.zeros(4, 8, 8, device="cuda"))
+        elif kind == "wrapped":
+            entry(Wrapped(torch.zeros(4, 8, 8), "cuda"))
+        else:
+            torch.func.grad(entry)(torch.zeros(4, 8, 8))
+    assert not flags
