@@ -30,6 +30,10 @@ void own_memory(const char* name, const Tensor& t) {
 void own_memory(const char* name, const OptTensor& t) { if (t.has_value()) own_memory(name, *t); }
 void own_memory(const char* name, at::TensorList list) { for (const Tensor& t : list) own_memory(name, t); }
 
+// A negated view (the imaginary part of a conjugate) holds its values with the other sign: they are written out.
+Tensor values(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor values(const OptTensor& t) { return t.has_value() ? values(*t) : Tensor(); }
+
 void first_order_only(const char* name) { TORCH_CHECK(!at::GradMode::is_enabled(), name, ": a gradient of the gradient is not available"); }
 
 // ---- layer norm ---------------------------------------------------------------------------------------------------------------
@@ -49,22 +53,22 @@ struct LayerNormBackward : public Node {
     own_memory("layer_norm", grads[0]);
     auto self = shared_from_this();
     const Tensor xs = x.unpack(self), ws = w.unpack(self);
-    auto out = layer_norm_bwd(grads[0], xs, optional_of(ws), b, stats, task_should_compute_output(0), ws.defined() && task_should_compute_output(1),
+    auto out = layer_norm_bwd(values(grads[0]), xs, optional_of(ws), b, stats, task_should_compute_output(0), ws.defined() && task_should_compute_output(1),
                               b.has_value() && task_should_compute_output(2));
     return {out[0], out[1], out[2]};
   }
 };
 
-Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, c10::optional<at::ScalarType> out_type) {
-  own_memory("layer_norm", x);
+Tensor layer_norm(const Tensor& x_, const OptTensor& w, const OptTensor& b, double eps, c10::optional<at::ScalarType> out_type) {
+  own_memory("layer_norm", x_);
   own_memory("layer_norm", w);
   own_memory("layer_norm", b);
-  const Tensor wt = w.value_or(Tensor()), bt = b.value_or(Tensor());
+  const Tensor x = values(x_), wt = values(w), bt = values(b);
   const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(wt) || wants_grad(bt));
   Tensor y, stats;
   {
     const at::NoGradGuard none;
-    std::tie(y, stats) = layer_norm_fwd(x, w, b, eps, out_type.value_or(x.scalar_type()), grad);
+    std::tie(y, stats) = layer_norm_fwd(x, optional_of(wt), optional_of(bt), eps, out_type.value_or(x.scalar_type()), grad);
   }
   if (grad) {
     auto node = std::shared_ptr<LayerNormBackward>(new LayerNormBackward(), torch::autograd::deleteNode);
@@ -72,7 +76,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, doubl
     node->x = SavedVariable(x, false);
     node->w = SavedVariable(wt, false);
     node->stats = stats;
-    if (b.has_value()) node->b = b->detach();
+    if (bt.defined()) node->b = bt.detach();
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -91,7 +95,7 @@ struct RotaryBackward : public Node {
   variable_list apply(variable_list&& grads) override {
     const std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("rotary");
-    const Tensor dq = task_should_compute_output(0) ? grads[0] : Tensor(), dk = grads.size() > 1 && task_should_compute_output(1) ? grads[1] : Tensor();
+    const Tensor dq = task_should_compute_output(0) ? values(grads[0]) : Tensor(), dk = grads.size() > 1 && task_should_compute_output(1) ? values(grads[1]) : Tensor();
     if (!dq.defined() && !dk.defined()) return variable_list(2);
     own_memory("rotary", grads);
     auto out = rotary_apply(dq, dk, pos.unpack(), freq.unpack(), magnitude, interleaved, -1.0);
@@ -99,12 +103,11 @@ struct RotaryBackward : public Node {
   }
 };
 
-std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& pos, const Tensor& frequencies, double magnitude, bool interleaved) {
-  for (const Tensor* t : {&q, &pos, &frequencies}) own_memory("rotary", *t);
+std::vector<Tensor> rotary(const Tensor& q_, const OptTensor& k, const Tensor& pos_, const Tensor& frequencies, double magnitude, bool interleaved) {
+  for (const Tensor* t : {&q_, &pos_, &frequencies}) own_memory("rotary", *t);
   own_memory("rotary", k);
-  const Tensor freq = frequencies.is_contiguous() ? frequencies : frequencies.contiguous();
-  rotary_check(q, k, pos, freq);
-  const Tensor kt = k.value_or(Tensor());
+  const Tensor q = values(q_), kt = values(k), pos = values(pos_), signed_freq = values(frequencies), freq = signed_freq.is_contiguous() ? signed_freq : signed_freq.contiguous();
+  rotary_check(q, optional_of(kt), pos, freq);
   const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(kt));
   std::pair<Tensor, Tensor> out;
   {
@@ -143,7 +146,7 @@ struct VocabLossBackward : public Node {
     if (!grads[0].defined()) return variable_list(2);
     own_memory("vocabulary_cross_entropy", grads[0]);
     const Tensor h = hidden.unpack(), w = weight.unpack(), t = target.unpack();
-    const Tensor g = grads[0].scalar_type() == at::kFloat && grads[0].is_contiguous() ? grads[0] : grads[0].to(at::kFloat).contiguous();
+    const Tensor given = values(grads[0]), g = given.scalar_type() == at::kFloat && given.is_contiguous() ? given : given.to(at::kFloat).contiguous();
     const bool want_dw = task_should_compute_output(1);
     Tensor buffer;
     if (want_dw && parameter.defined()) {
@@ -156,8 +159,9 @@ struct VocabLossBackward : public Node {
 };
 
 // hidden [..., h]; weight [vocabulary, h] and the same in bf16; target of hidden's leading shape.
-Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weight16, const Tensor& target, int64_t reduction, bool managed, int64_t workspace, const Tensor& err) {
-  for (const Tensor* t : {&hidden, &weight, &weight16, &target, &err}) own_memory("vocabulary_cross_entropy", *t);
+Tensor vocab_loss(const Tensor& hidden_, const Tensor& weight, const Tensor& weight16, const Tensor& target_, int64_t reduction, bool managed, int64_t workspace, const Tensor& err) {
+  for (const Tensor* t : {&hidden_, &weight, &weight16, &target_, &err}) own_memory("vocabulary_cross_entropy", *t);
+  const Tensor hidden = values(hidden_), target = values(target_);
   TORCH_CHECK_VALUE(weight.dim() == 2 && hidden.dim() >= 1 && hidden.size(-1) == weight.size(1) && weight.numel() > 0,
                     "vocabulary_cross_entropy: hidden [..., h] and weight [vocabulary, h] required");
   TORCH_CHECK_VALUE(target.sizes() == hidden.sizes().slice(0, hidden.dim() - 1) && target.scalar_type() == at::kLong, "vocabulary_cross_entropy: int64 targets of hidden's leading shape required");
@@ -171,7 +175,7 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weig
     // Views of what was given where nothing has to be converted or copied: a change before the backward is then noticed.  Copies into padded rows are kept for it.
     h = hidden.scalar_type() == at::kBFloat16 ? hidden : hidden.to(at::kBFloat16);
     h = vocab_rows(h.dim() == 2 ? h : h.reshape({-1, h.size(-1)}));
-    w = vocab_rows(weight16);
+    w = vocab_rows(values(weight16));
     t = target.dim() == 1 ? target : target.reshape({-1});
     if (!t.is_contiguous()) t = t.contiguous();
     auto out = vocab_loss_fwd(h, w, t, target.sizes(), reduction, err);
@@ -196,7 +200,15 @@ Tensor vocab_loss(const Tensor& hidden, const Tensor& weight, const Tensor& weig
 Tensor clip(const char* name, at::TensorList grads, at::TensorList outs, double max_norm, bool scale) {
   own_memory(name, grads);
   own_memory(name, outs);
-  return clip_grad_norm(grads, outs, max_norm, scale);
+  // the norm and the scaling in place are the same for either sign; a result of the other sign takes its gradient's values with that sign
+  const at::NoGradGuard none;
+  std::vector<Tensor> turned;
+  for (size_t i = 0; i < outs.size() && i < grads.size(); ++i)
+    if (outs[i].is_neg() != grads[i].is_neg()) {
+      if (turned.empty()) turned = grads.vec();
+      turned[i] = outs[i].is_neg() ? grads[i].neg() : grads[i].resolve_neg();
+    }
+  return clip_grad_norm(turned.empty() ? grads : at::TensorList(turned), outs, max_norm, scale);
 }
 
 }  // namespace

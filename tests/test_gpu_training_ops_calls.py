@@ -120,3 +120,33 @@ def test_batched_gradients_are_refused(which):
 def test_layer_norm_under_vmap():
     x = torch.randn(3, 5, 64, device="cuda")
     assert torch.equal(torch.func.vmap(ops.layer_norm)(x), ops.layer_norm(x))
+
+
+# ---- views with the other sign -----------------------------------------------------------------------------------------------------------
+def negated(t):
+    """The same values, as the imaginary part of a conjugate is held: in memory with the other sign, a bit saying so."""
+    return torch._neg_view(-t)
+
+
+def test_negated_views_have_their_values():
+    x, w, b, dy = (torch.randn(*s, device="cuda") for s in ((6, 64), (64,), (64,), (6, 64)))
+    assert negated(x).is_neg() and torch.equal(negated(x) + 0, x)
+    want, got = [], []
+    for out, wrap in ((want, lambda t: t), (got, negated)):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = ops.layer_norm(*(wrap(t) for t in leaves))
+        out += [y, *torch.autograd.grad(y, leaves, wrap(dy))]
+        q, k = (torch.randn(2, 6, n, 16, device="cuda", generator=torch.Generator("cuda").manual_seed(n)).requires_grad_() for n in (4, 2))
+        freq, _ = ops.rotary_frequencies(16, device="cuda")
+        turned = ops.rotary(wrap(q), wrap(k), torch.arange(6, device="cuda"), wrap(freq))
+        out += [*turned, *torch.autograd.grad(turned, [q, k], [wrap(q.detach()), wrap(k.detach())])]
+        h, m, target = master(6)
+        losses = vocabulary_cross_entropy(wrap(m), wrap(h), target, "none")
+        out += [losses, *torch.autograd.grad(losses, [h, m], wrap(losses.detach()))]
+        mean = vocabulary_cross_entropy(wrap(m.detach().to(BF16)), h, target)
+        out += [mean, *torch.autograd.grad(mean, h, wrap(torch.ones_like(mean)))]
+        grads = [x.clone(), w.clone()]
+        out += [ops.grad_norm([wrap(g) for g in grads]), ops.clip_grad_norm([wrap(g) for g in grads], 1.0, out=(into := [torch.empty_like(g) for g in grads])), *into]
+        grads = [wrap(g) for g in grads]
+        out += [ops.clip_grad_norm(grads, 1.0), *(g + 0 for g in grads)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
