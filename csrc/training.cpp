@@ -21,14 +21,15 @@ bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
 // The entries are registered for every kind of tensor, and the kernels take addresses: a fake or wrapped tensor has a null one (a launch would fault), a batched or
-// transformed one none of its own.
-void own_memory(const char* name, const Tensor& t) {
+// transformed one none of its own.  A tensor with a tangent (forward mode) would give a result without one, which counts as a constant.
+void check_operand(const char* name, const Tensor& t) {
   constexpr c10::DispatchKeySet without{c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchGradWrapper,
                                         c10::DispatchKey::ZeroTensor};
   TORCH_CHECK_VALUE(!t.defined() || !t.key_set().has_any(without), name, ": a tensor with values in memory of its own is required, not one that is fake, wrapped, batched or transformed");
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), name, ": derivatives in forward mode are not available");
 }
-void own_memory(const char* name, const OptTensor& t) { if (t.has_value()) own_memory(name, *t); }
-void own_memory(const char* name, at::TensorList list) { for (const Tensor& t : list) own_memory(name, t); }
+void check_operand(const char* name, const OptTensor& t) { if (t.has_value()) check_operand(name, *t); }
+void check_operand(const char* name, at::TensorList list) { for (const Tensor& t : list) check_operand(name, t); }
 
 // A negated view (the imaginary part of a conjugate) holds its values with the other sign: they are written out.
 Tensor values(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
@@ -50,7 +51,7 @@ struct LayerNormBackward : public Node {
     const std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("layer_norm");
     if (!grads[0].defined()) return variable_list(3);
-    own_memory("layer_norm", grads[0]);
+    check_operand("layer_norm", grads[0]);
     auto self = shared_from_this();
     const Tensor xs = x.unpack(self), ws = w.unpack(self);
     auto out = layer_norm_bwd(values(grads[0]), xs, optional_of(ws), b, stats, task_should_compute_output(0), ws.defined() && task_should_compute_output(1),
@@ -60,9 +61,9 @@ struct LayerNormBackward : public Node {
 };
 
 Tensor layer_norm(const Tensor& x_, const OptTensor& w, const OptTensor& b, double eps, c10::optional<at::ScalarType> out_type) {
-  own_memory("layer_norm", x_);
-  own_memory("layer_norm", w);
-  own_memory("layer_norm", b);
+  check_operand("layer_norm", x_);
+  check_operand("layer_norm", w);
+  check_operand("layer_norm", b);
   const Tensor x = values(x_), wt = values(w), bt = values(b);
   const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(wt) || wants_grad(bt));
   Tensor y, stats;
@@ -97,15 +98,15 @@ struct RotaryBackward : public Node {
     first_order_only("rotary");
     const Tensor dq = task_should_compute_output(0) ? values(grads[0]) : Tensor(), dk = grads.size() > 1 && task_should_compute_output(1) ? values(grads[1]) : Tensor();
     if (!dq.defined() && !dk.defined()) return variable_list(2);
-    own_memory("rotary", grads);
+    check_operand("rotary", grads);
     auto out = rotary_apply(dq, dk, pos.unpack(), freq.unpack(), magnitude, interleaved, -1.0);
     return {out.first, out.second};
   }
 };
 
 std::vector<Tensor> rotary(const Tensor& q_, const OptTensor& k, const Tensor& pos_, const Tensor& frequencies, double magnitude, bool interleaved) {
-  for (const Tensor* t : {&q_, &pos_, &frequencies}) own_memory("rotary", *t);
-  own_memory("rotary", k);
+  for (const Tensor* t : {&q_, &pos_, &frequencies}) check_operand("rotary", *t);
+  check_operand("rotary", k);
   const Tensor q = values(q_), kt = values(k), pos = values(pos_), signed_freq = values(frequencies), freq = signed_freq.is_contiguous() ? signed_freq : signed_freq.contiguous();
   rotary_check(q, optional_of(kt), pos, freq);
   const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(kt));
@@ -144,7 +145,7 @@ struct VocabLossBackward : public Node {
     const std::lock_guard<std::mutex> lock(mutex_);
     first_order_only("vocabulary_cross_entropy");
     if (!grads[0].defined()) return variable_list(2);
-    own_memory("vocabulary_cross_entropy", grads[0]);
+    check_operand("vocabulary_cross_entropy", grads[0]);
     const Tensor h = hidden.unpack(), w = weight.unpack(), t = target.unpack();
     const Tensor given = values(grads[0]), g = given.scalar_type() == at::kFloat && given.is_contiguous() ? given : given.to(at::kFloat).contiguous();
     const bool want_dw = task_should_compute_output(1);
@@ -160,7 +161,7 @@ struct VocabLossBackward : public Node {
 
 // hidden [..., h]; weight [vocabulary, h] and the same in bf16; target of hidden's leading shape.
 Tensor vocab_loss(const Tensor& hidden_, const Tensor& weight, const Tensor& weight16, const Tensor& target_, int64_t reduction, bool managed, int64_t workspace, const Tensor& err) {
-  for (const Tensor* t : {&hidden_, &weight, &weight16, &target_, &err}) own_memory("vocabulary_cross_entropy", *t);
+  for (const Tensor* t : {&hidden_, &weight, &weight16, &target_, &err}) check_operand("vocabulary_cross_entropy", *t);
   const Tensor hidden = values(hidden_), target = values(target_);
   TORCH_CHECK_VALUE(weight.dim() == 2 && hidden.dim() >= 1 && hidden.size(-1) == weight.size(1) && weight.numel() > 0,
                     "vocabulary_cross_entropy: hidden [..., h] and weight [vocabulary, h] required");
@@ -198,8 +199,8 @@ Tensor vocab_loss(const Tensor& hidden_, const Tensor& weight, const Tensor& wei
 }
 
 Tensor clip(const char* name, at::TensorList grads, at::TensorList outs, double max_norm, bool scale) {
-  own_memory(name, grads);
-  own_memory(name, outs);
+  check_operand(name, grads);
+  check_operand(name, outs);
   // the norm and the scaling in place are the same for either sign; a result of the other sign takes its gradient's values with that sign
   const at::NoGradGuard none;
   std::vector<Tensor> turned;
@@ -222,5 +223,5 @@ TORCH_LIBRARY_FRAGMENT(q38, m) {
   m.def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm) -> Tensor", [](at::TensorList g, double m) { return q38::clip("clip_grad_norm", g, {}, m, true); });
   m.def("clip_grad_norm_out(Tensor[] grads, Tensor(a!)[] out, float max_norm) -> Tensor",
         [](at::TensorList g, at::TensorList o, double m) { return q38::clip("clip_grad_norm", g, o, m, true); });
-  m.def("own_memory(Tensor[] tensors, str name) -> ()", [](at::TensorList t, c10::string_view name) { q38::own_memory(std::string(name).c_str(), t); });
+  m.def("check_operands(Tensor[] tensors, str name) -> ()", [](at::TensorList t, c10::string_view name) { q38::check_operand(std::string(name).c_str(), t); });
 }

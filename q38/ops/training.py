@@ -1,7 +1,7 @@
 """Operators around the products of a training step: layer norm, rotary positions, and the global gradient norm with clipping.
 
 On a GPU each runs on the kernels of `csrc/layernorm.cu`, `csrc/rotary.cu` and `csrc/clip.cu` (current stream of the tensors' device; capturable into a
-CUDA graph; first derivatives only; fake and wrapped tensors are refused, so a sharded one goes in as its local part); tensors in host memory take the plain
+CUDA graph; first derivatives only, backward; fake and wrapped tensors are refused, so a sharded one goes in as its local part); tensors in host memory take the plain
 PyTorch formulas below, which are the specification.
 """
 import math

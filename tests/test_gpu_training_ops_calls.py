@@ -150,3 +150,31 @@ def test_negated_views_have_their_values():
         grads = [wrap(g) for g in grads]
         out += [ops.clip_grad_norm(grads, 1.0), *(g + 0 for g in grads)]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- derivatives that are not offered ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("call", [
+    lambda t: ops.layer_norm(t), lambda t: ops.layer_norm(t.detach(), t[0]), lambda t: ops.layer_norm(t.detach(), None, t[0]),
+    lambda t: ops.rotary(t.view(1, 6, 4, 16), None, torch.arange(6, device="cuda"), ops.rotary_frequencies(16, device="cuda")[0]),
+    lambda t: ops.rotary(t.detach().view(6, 4, 16), t.view(6, 4, 16), torch.arange(6, device="cuda"), ops.rotary_frequencies(16, device="cuda")[0]),
+    lambda t: ops.rotary(t.detach().view(6, 4, 16), None, torch.arange(6, device="cuda"), t[0, :8].double()),
+    lambda t: vocabulary_cross_entropy(t.detach(), t, torch.arange(6, device="cuda")), lambda t: vocabulary_cross_entropy(t, t.detach(), torch.arange(6, device="cuda")),
+    lambda t: ops.grad_norm([t]), lambda t: ops.clip_grad_norm([t], 1.0), lambda t: ops.clip_grad_norm([t], 1.0, out=[t.detach().clone()]),
+    lambda t: ops.clip_grad_norm([t.detach().clone()], 1.0, out=[t]),
+])
+def test_forward_mode_is_refused(call):
+    x = torch.randn(6, 64, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        t = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            call(t)
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.func.jvp(call, (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.parametrize("which", range(3))
+def test_gradients_with_a_tangent_are_refused(which):
+    y, leaf = outputs()[which]
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward mode"):
+            torch.autograd.grad(y, leaf, torch.autograd.forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))

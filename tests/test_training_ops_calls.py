@@ -12,7 +12,7 @@ class Native:
     def __init__(self):
         self.weights = []
 
-    def own_memory(self, tensors, name):
+    def check_operands(self, tensors, name):
         pass
 
     def vocab_loss(self, hidden, weight, weight16, target, reduction, managed, workspace, err):
@@ -151,3 +151,13 @@ def test_tensors_without_memory_are_refused(entry, kind, monkeypatch):
         else:
             torch.func.grad(entry)(torch.zeros(4, 8, 8))
     assert not flags
+
+
+# ---- derivatives that are not offered ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("entry", [e for e in ENTRIES if e not in (_turned_at, _losses_of)])
+def test_forward_mode_is_refused(entry):
+    """A result without a tangent would be taken for a constant."""
+    x = torch.zeros(4, 8, 8)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward mode"):
+            entry(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
