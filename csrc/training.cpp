@@ -107,6 +107,7 @@ struct RotaryBackward : public Node {
 std::vector<Tensor> rotary(const Tensor& q_, const OptTensor& k, const Tensor& pos_, const Tensor& frequencies, double magnitude, bool interleaved) {
   for (const Tensor* t : {&q_, &pos_, &frequencies}) check_operand("rotary", *t);
   check_operand("rotary", k);
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && frequencies.requires_grad()), "rotary: a gradient of the frequencies is not available; detached ones are required");
   const Tensor q = values(q_), kt = values(k), pos = values(pos_), signed_freq = values(frequencies), freq = signed_freq.is_contiguous() ? signed_freq : signed_freq.contiguous();
   rotary_check(q, optional_of(kt), pos, freq);
   const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(kt));

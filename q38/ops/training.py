@@ -103,7 +103,7 @@ def rotary(q, k, positions, frequencies, magnitude=1.0, interleaved=False):
     q: ``[batch, seq, heads, dim]`` or ``[tokens, heads, dim]``; k: the same with a head count of its own, or None.  bf16, fp16 or fp32, any strides (a head-major
     tensor goes in as ``x.transpose(1, 2)``, a packed projection as slices); results have the layout of their input.  positions: whole numbers ``[seq]``
     or ``[batch, seq]`` (``[tokens]``), of any size and sign; angles are formed in 64 bits.  frequencies: ``rotary_dim / 2`` values in 64 bits
-    (`rotary_frequencies`); dimensions from rotary_dim on pass through.  A pair is ``(x[i], x[i + rotary_dim / 2])``, interleaved ``(x[2 i], x[2 i + 1])``."""
+    (`rotary_frequencies`), which get no gradient: ones that want it are refused; dimensions from rotary_dim on pass through.  A pair is ``(x[i], x[i + rotary_dim / 2])``, interleaved ``(x[2 i], x[2 i + 1])``."""
     if q.dim() == 3:
         _require(k is None or k.dim() == 3, "rotary: queries and keys have the same number of dimensions")
         q2, k2 = rotary(q.unsqueeze(0), None if k is None else k.unsqueeze(0), positions, frequencies, magnitude, interleaved)
@@ -120,6 +120,7 @@ def rotary(q, k, positions, frequencies, magnitude=1.0, interleaved=False):
              "rotary: whole positions [seq] or [batch, seq] on the queries' device required")
     _require(frequencies.dtype == torch.float64 and frequencies.device == q.device and frequencies.dim() == 1 and 2 * frequencies.shape[0] <= D,
              "rotary: 64-bit frequencies on the queries' device, at most half a head of them, required")
+    _require(not (torch.is_grad_enabled() and frequencies.requires_grad), "rotary: a gradient of the frequencies is not available; detached ones are required")
     angle = positions.double()[..., None, None] * frequencies
     cos, sin = (angle.cos() * magnitude).float(), (angle.sin() * magnitude).float()
     return _rotate(q, cos, sin, interleaved), None if k is None else _rotate(k, cos, sin, interleaved)

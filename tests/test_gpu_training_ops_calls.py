@@ -178,3 +178,16 @@ def test_gradients_with_a_tangent_are_refused(which):
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward mode"):
             torch.autograd.grad(y, leaf, torch.autograd.forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_a_gradient_of_the_frequencies_is_refused():
+    q = torch.randn(1, 6, 2, 16, device="cuda", requires_grad=True)
+    freq, _ = ops.rotary_frequencies(16, device="cuda")
+    learned, pos = freq.clone().requires_grad_(), torch.arange(6, device="cuda")
+    for arg in (q, q.detach()):
+        with pytest.raises(ValueError, match="frequencies"):
+            ops.rotary(arg, None, pos, learned)
+    want = ops.rotary(q, None, pos, freq)[0]
+    with torch.no_grad():
+        assert torch.equal(ops.rotary(q, None, pos, learned)[0], want)
+    assert torch.equal(ops.rotary(q, None, pos, learned.detach())[0], want)

@@ -161,3 +161,25 @@ def test_forward_mode_is_refused(entry):
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward mode"):
             entry(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+def _learned(k=True, device="cpu"):
+    q = torch.randn(1, 4, 2, 8, device=device, requires_grad=True)
+    f = torch.rand(4, dtype=torch.float64, device=device).requires_grad_()
+    return lambda: ops.rotary(q, q.detach() if k else None, torch.arange(4, device=device), f)
+
+
+@pytest.mark.parametrize("k", [True, False])
+def test_a_gradient_of_the_frequencies_is_refused(k):
+    """Neither device offers one, so that neither leaves a learned vector without one unnoticed."""
+    call = _learned(k)
+    with pytest.raises(ValueError, match="frequencies"):
+        call()
+    with torch.no_grad():
+        call()
+
+
+def test_a_gradient_of_the_frequencies_is_refused_where_the_kernel_is_called():
+    q, f = torch.zeros(1, 4, 2, 8), torch.zeros(4, dtype=torch.float64, requires_grad=True)
+    with pytest.raises(ValueError, match="frequencies"):
+        ops.load().rotary(q, None, torch.arange(4), f, 1.0, False)
