@@ -17,6 +17,7 @@
 #include "ptx.cuh"
 #include "host.h"
 #include "launch.cuh"
+#include "shared_memory.h"
 #include "training.h"
 
 namespace q38 {
@@ -423,6 +424,13 @@ static void gemm_p(const at::Tensor& a_, const at::Tensor& b_, const at::Tensor&
     if (b_mn_major) launch_p<false, true>(ta, tb, tc, tma_out, p, out_fp32, accumulate, stream);
     else launch_p<false, false>(ta, tb, tc, tma_out, p, out_fp32, accumulate, stream);
   }
+}
+
+void allow_shared_memory(const void* kernel, int bytes) {
+  static SharedMemoryGrants grants;
+  int device = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&device));
+  grants.ensure(kernel, device, bytes, [&] { C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)); });
 }
 
 // Same contract as gemm_bf16 (bf16 operands only).

@@ -14,9 +14,6 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
-#include <mutex>
-#include <set>
-
 #include "f32x2.cuh"
 #include "packs.cuh"
 #include "host.h"
@@ -569,17 +566,6 @@ struct Rows {
 };
 
 }  // namespace
-
-void allow_shared_memory(const void* kernel, int bytes) {
-  static std::mutex mutex;
-  static std::set<std::pair<const void*, int>> done;
-  int device = 0;
-  C10_CUDA_CHECK(cudaGetDevice(&device));
-  const std::lock_guard<std::mutex> lock(mutex);
-  if (done.count({kernel, device})) return;
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  done.insert({kernel, device});
-}
 
 std::pair<at::Tensor, at::Tensor> layer_norm_fwd(const at::Tensor& x, const OptTensor& w, const OptTensor& b, double eps, at::ScalarType out_type, bool save) {
   TORCH_CHECK_VALUE(x.is_cuda() && x.dim() > 0 && x.size(-1) > 0 && x.size(-1) <= INT_MAX / 2, "layer_norm: a CUDA input with a last dimension that is not empty is required");

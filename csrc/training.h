@@ -12,7 +12,7 @@ using OptTensor = c10::optional<at::Tensor>;
 // A CUDA tensor without the dispatcher's way, which costs a short call as much as its kernel's launch.
 inline at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType type, at::Device device) { return at::detail::empty_cuda(sizes, type, device, c10::nullopt); }
 
-// Lets `kernel` take `bytes` of dynamic shared memory on the current device; the driver is asked once per kernel and device.
+// Lets `kernel` take `bytes` of dynamic shared memory on the current device; the driver is asked when a kernel and device need more than before (gemm_persistent.cu).
 void allow_shared_memory(const void* kernel, int bytes);
 
 // Any x with a last dimension -> {y of x's shape, [2, rows] mean and 1 / deviation (undefined without `save`)}.
