@@ -53,7 +53,7 @@ def vocabulary_cross_entropy(weight, hidden, target, reduction="mean"):
     if weight.device != hidden.device or target.device != hidden.device:
         raise ValueError("vocabulary_cross_entropy: hidden, weight and target on one device required")
     h2, t1 = hidden.reshape(-1, hidden.shape[-1]), target.reshape(-1)
-    scores = F.linear(h2, weight.to(h2.dtype)).float()
+    scores = F.linear(h2.float(), weight.to(h2.dtype).float())              # not in bf16: half a step of a score of ten is 2 % of a probability
     losses = F.cross_entropy(scores, t1, ignore_index=-100, reduction="none")
     if reduction == "none":
         return losses.view(target.shape)

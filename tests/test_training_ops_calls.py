@@ -183,3 +183,29 @@ def test_a_gradient_of_the_frequencies_is_refused_where_the_kernel_is_called():
     q, f = torch.zeros(1, 4, 2, 8), torch.zeros(4, dtype=torch.float64, requires_grad=True)
     with pytest.raises(ValueError, match="frequencies"):
         ops.load().rotary(q, None, torch.arange(4), f, 1.0, False)
+
+
+# ---- vocabulary loss in host memory --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("ht,wt", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
+def test_scores_of_the_vocabulary_loss_are_fp32(ht, wt):
+    """Scores of tens: one rounded to bf16 is off by 2^-9 of itself, which is a few per cent of a probability."""
+    from q38.losses import vocabulary_cross_entropy
+    gen = torch.Generator().manual_seed(0)
+    rows, words, width, u = 20, 300, 48, 2.0 ** -24
+    h, w = (torch.randn(rows, width, generator=gen) * 2).to(ht).requires_grad_(), torch.randn(words, width, generator=gen).to(wt).requires_grad_()
+    target = torch.randint(0, words, (rows,), generator=gen)
+    hd = h.detach().double().requires_grad_()
+    wd = w.detach().to(ht).double().requires_grad_()                        # a master weight is rounded as the hidden states are
+    want = torch.nn.functional.cross_entropy(hd @ wd.T, target, reduction="none")
+    got = vocabulary_cross_entropy(w, h, target, "none")
+    # a score has `width` additions; a loss the sum over the words, its logarithm and the target's score
+    score_off = (width + 2) * u * (hd.abs() @ wd.abs().T)
+    tol = 2 * score_off.amax(-1) + (words + 8) * u + 4 * u * (hd @ wd.T).abs().amax(-1)
+    assert got.dtype == torch.float32 and ((got - want).abs() <= tol).all()
+    # gradients: probabilities to twice that (relative), sums over words and rows, and half a step of the result's type
+    dz = torch.softmax(hd @ wd.T, -1) - torch.nn.functional.one_hot(target, words)
+    dz_off = (2 * tol[:, None] + 8 * u) * dz.abs() + 4 * u
+    dh, dw = torch.autograd.grad(got.sum(), [h, w])
+    for g, e, off in ((dh, dz @ wd, dz_off @ wd.abs() + words * u * (dz.abs() @ wd.abs())), (dw, dz.T @ hd, dz_off.T @ hd.abs() + rows * u * (dz.abs().T @ hd.abs()))):
+        kept = ht if g is dw and wt == torch.float32 else g.dtype           # a master weight's gradient passes through the type that it was rounded to
+        assert ((g.double() - e).abs() <= off + torch.finfo(kept).eps / 2 * (e.abs() + off)).all()
