@@ -298,6 +298,12 @@ def bench_ngram(rows, shape, T, iters, pk, seq=4096):
     report(rows, f"ngram_bwd T={T} h={h}", t, bytes_=T * h * (2.0 + 2 * 4 + 2 * 8), pk=pk)
 
 
+def sequences(tokens, longest=4096):
+    """Whole sequences of at most `longest` tokens out of `tokens`: how many, and their length."""
+    seq = min(tokens, longest)
+    return tokens // seq, seq
+
+
 def bench_training(rows, shape, T, iters, pk):
     """Layer norm, rotary positions, gradient clipping and the vocabulary loss in pieces, as `q38.ops` and `q38.losses` offer them (forward passes)."""
     from .. import ops
@@ -313,15 +319,16 @@ def bench_training(rows, shape, T, iters, pk):
 
     t = timeit(lambda: ops.layer_norm(turn(x), w, b), iters)
     report(rows, f"layer_norm T={T} h={h}", t, bytes_=4.0 * T * h, pk=pk)
-    qkv = [torch.randn(T // 4096, 4096, heads + 2 * kv, 64, device="cuda").to(torch.bfloat16) for _ in range(4)]
-    pos, (freq, magnitude) = torch.arange(4096, device="cuda"), ops.rotary_frequencies(16, shape["rope_theta"], device="cuda")
+    batch, seq = sequences(T)
+    qkv = [torch.randn(batch, seq, heads + 2 * kv, 64, device="cuda").to(torch.bfloat16) for _ in range(4)]
+    pos, (freq, magnitude) = torch.arange(seq, device="cuda"), ops.rotary_frequencies(16, shape["rope_theta"], device="cuda")
 
     def rotate():
         packed = turn(qkv)
         ops.rotary(packed[:, :, :heads], packed[:, :, heads:heads + kv], pos, freq, magnitude)
 
     t = timeit(rotate, iters)
-    report(rows, f"rotary T={T} heads={heads}+{kv}", t, bytes_=4.0 * (T // 4096 * 4096) * (heads + kv) * 64, pk=pk)
+    report(rows, f"rotary T={batch * seq} heads={heads}+{kv}", t, bytes_=4.0 * batch * seq * (heads + kv) * 64, pk=pk)
     grads = [torch.randn(2_000_000, device="cuda") for _ in range(60)]
     out = [torch.empty_like(g) for g in grads]
     t = timeit(lambda: ops.clip_grad_norm(grads, 1.0, out=out), iters)

@@ -191,3 +191,14 @@ def test_a_gradient_of_the_frequencies_is_refused():
     with torch.no_grad():
         assert torch.equal(ops.rotary(q, None, pos, learned)[0], want)
     assert torch.equal(ops.rotary(q, None, pos, learned.detach())[0], want)
+
+
+# ---- the kernel bench ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens,turned", [(100, 100), (5000, 4096)])
+def test_kernel_bench_labels_what_ran(tokens, turned):
+    from q38.utils.kernel_bench import bench_training
+    rows = []
+    bench_training(rows, dict(hidden=64, heads=3, kv_heads=1, rope_theta=1e6), tokens, 1, dict(tflops=1.0, hbm_gbs=1.0, source="test"))
+    row, = [r for r in rows if r["kernel"].startswith("rotary")]
+    assert row["kernel"] == f"rotary T={turned} heads=3+1"
+    assert abs(row["gbs"] * row["us"] * 1e3 / (4 * turned * 4 * 64) - 1) < 1e-6

@@ -209,3 +209,9 @@ def test_scores_of_the_vocabulary_loss_are_fp32(ht, wt):
     for g, e, off in ((dh, dz @ wd, dz_off @ wd.abs() + words * u * (dz.abs() @ wd.abs())), (dw, dz.T @ hd, dz_off.T @ hd.abs() + rows * u * (dz.abs().T @ hd.abs()))):
         kept = ht if g is dw and wt == torch.float32 else g.dtype           # a master weight's gradient passes through the type that it was rounded to
         assert ((g.double() - e).abs() <= off + torch.finfo(kept).eps / 2 * (e.abs() + off)).all()
+
+
+# ---- the kernel bench ----------------------------------------------------------------------------------------------------------------------
+def test_kernel_bench_sequences():
+    from q38.utils.kernel_bench import sequences
+    assert [sequences(t) for t in (1, 100, 4095, 4096, 10000, 16384)] == [(1, 1), (1, 100), (1, 4095), (1, 4096), (2, 4096), (4, 4096)]
