@@ -2,6 +2,7 @@
 // per pass, torch's own wrapper for C++ functions half of that, and the kernels of a short sequence take 2 to 5.
 #include <ATen/ATen.h>
 #include <c10/core/DispatchKeySet.h>
+#include <c10/core/InferenceMode.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -17,6 +18,8 @@ using torch::autograd::Node;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
+// Gradients enabled inside inference mode are not recorded
+bool recording() { return at::GradMode::is_enabled() && !c10::InferenceMode::is_enabled(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 
@@ -65,7 +68,7 @@ Tensor layer_norm(const Tensor& x_, const OptTensor& w, const OptTensor& b, doub
   check_operand("layer_norm", w);
   check_operand("layer_norm", b);
   const Tensor x = values(x_), wt = values(w), bt = values(b);
-  const bool grad = at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(wt) || wants_grad(bt));
+  const bool grad = recording() && (wants_grad(x) || wants_grad(wt) || wants_grad(bt));
   Tensor y, stats;
   {
     const at::NoGradGuard none;
@@ -107,10 +110,10 @@ struct RotaryBackward : public Node {
 std::vector<Tensor> rotary(const Tensor& q_, const OptTensor& k, const Tensor& pos_, const Tensor& frequencies, double magnitude, bool interleaved) {
   for (const Tensor* t : {&q_, &pos_, &frequencies}) check_operand("rotary", *t);
   check_operand("rotary", k);
-  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && frequencies.requires_grad()), "rotary: a gradient of the frequencies is not available; detached ones are required");
+  TORCH_CHECK_VALUE(!(recording() && frequencies.requires_grad()), "rotary: a gradient of the frequencies is not available; detached ones are required");
   const Tensor q = values(q_), kt = values(k), pos = values(pos_), signed_freq = values(frequencies), freq = signed_freq.is_contiguous() ? signed_freq : signed_freq.contiguous();
   rotary_check(q, optional_of(kt), pos, freq);
-  const bool grad = at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(kt));
+  const bool grad = recording() && (wants_grad(q) || wants_grad(kt));
   std::pair<Tensor, Tensor> out;
   {
     const at::NoGradGuard none;                                    // layouts that need a copy
@@ -170,7 +173,7 @@ Tensor vocab_loss(const Tensor& hidden_, const Tensor& weight, const Tensor& wei
   for (const Tensor* t : {&hidden, &weight})
     TORCH_CHECK_VALUE(t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat, "vocabulary_cross_entropy: bf16 or fp32 hidden states and weight required");
   TORCH_CHECK_VALUE(hidden.is_cuda() && weight.device() == hidden.device() && target.device() == hidden.device(), "vocabulary_cross_entropy: hidden, weight and target on one device required");
-  const bool grad = at::GradMode::is_enabled() && (wants_grad(hidden) || wants_grad(weight));
+  const bool grad = recording() && (wants_grad(hidden) || wants_grad(weight));
   Tensor h, w, t, loss, lse2, count;
   {
     const at::NoGradGuard none;

@@ -120,7 +120,7 @@ def rotary(q, k, positions, frequencies, magnitude=1.0, interleaved=False):
              "rotary: whole positions [seq] or [batch, seq] on the queries' device required")
     _require(frequencies.dtype == torch.float64 and frequencies.device == q.device and frequencies.dim() == 1 and 2 * frequencies.shape[0] <= D,
              "rotary: 64-bit frequencies on the queries' device, at most half a head of them, required")
-    _require(not (torch.is_grad_enabled() and frequencies.requires_grad), "rotary: a gradient of the frequencies is not available; detached ones are required")
+    _require(not (torch.is_grad_enabled() and not torch.is_inference_mode_enabled() and frequencies.requires_grad), "rotary: a gradient of the frequencies is not available; detached ones are required")
     angle = positions.double()[..., None, None] * frequencies
     cos, sin = (angle.cos() * magnitude).float(), (angle.sin() * magnitude).float()
     return _rotate(q, cos, sin, interleaved), None if k is None else _rotate(k, cos, sin, interleaved)

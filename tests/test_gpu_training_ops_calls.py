@@ -202,3 +202,20 @@ def test_kernel_bench_labels_what_ran(tokens, turned):
     row, = [r for r in rows if r["kernel"].startswith("rotary")]
     assert row["kernel"] == f"rotary T={turned} heads=3+1"
     assert abs(row["gbs"] * row["us"] * 1e3 / (4 * turned * 4 * 64) - 1) < 1e-6
+
+
+# ---- inference mode ------------------------------------------------------------------------------------------------------------------------
+def test_gradients_enabled_inside_inference_mode_are_not_recorded():
+    """As for torch's own operators: inference mode comes before `enable_grad`."""
+    x = torch.randn(6, 64, device="cuda", requires_grad=True)
+    q = torch.randn(1, 6, 2, 16, device="cuda", requires_grad=True)
+    h, w, target = master(7, 6, 100)
+    freq, pos = ops.rotary_frequencies(16, device="cuda")[0], torch.arange(6, device="cuda")
+    calls = [lambda: ops.layer_norm(x), lambda: ops.rotary(q, None, pos, freq)[0], lambda: ops.rotary(q, None, pos, freq.clone().requires_grad_())[0],
+             lambda: vocabulary_cross_entropy(w, h, target), lambda: vocabulary_cross_entropy(w.detach().to(BF16), h, target, "none")]
+    want = [ops.layer_norm(x), *[ops.rotary(q, None, pos, freq)[0]] * 2, vocabulary_cross_entropy(w, h, target), vocabulary_cross_entropy(w, h, target, "none")]
+    for call, value in zip(calls, want):
+        with torch.inference_mode(), torch.enable_grad():
+            got = call()
+            assert not got.requires_grad and got.is_inference()
+        assert torch.equal(got, value)
