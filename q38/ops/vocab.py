@@ -15,7 +15,10 @@ def vocabulary_loss(hidden, weight, target, reduction):
     a training pass): a copy kept on the weight would be missing from a captured graph, unordered on a second stream and stale after a change through `.data`."""
     lib = load()
     if hidden.device.index not in _error_flags:
-        lib.check_operands([hidden, weight, target], "vocabulary_cross_entropy")   # before the device's error word is made and kept, which would be no memory either
+        # the device's error word is about to be made and kept: not as a fake tensor, and not by a graph, whose replays would write its zeros
+        lib.check_operands([hidden, weight, target], "vocabulary_cross_entropy")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("vocabulary_cross_entropy: call it once on this device (or q38.ops.install()) before it is captured")
     shadow = getattr(weight, "_q38_bf16", None)
     weight16 = shadow if shadow is not None else weight.detach().to(torch.bfloat16)
     return lib.vocab_loss(hidden, weight, weight16, target, REDUCTIONS[reduction], shadow is not None, PIECE_BYTES, error_flag(hidden.device))

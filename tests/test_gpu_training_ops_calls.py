@@ -219,3 +219,27 @@ def test_gradients_enabled_inside_inference_mode_are_not_recorded():
             got = call()
             assert not got.requires_grad and got.is_inference()
         assert torch.equal(got, value)
+
+
+def test_a_first_call_is_not_captured(monkeypatch):
+    h, w, target = master(8, 6, 100)
+    with monkeypatch.context() as m:
+        m.setattr(ops, "_error_flags", flags := {})
+        m.setattr("q38.ops.vocab._error_flags", flags)
+        with pytest.raises(RuntimeError, match="before it is captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                vocabulary_cross_entropy(w, h, target)
+        assert not flags
+        want = vocabulary_cross_entropy(w, h, target)
+        assert list(flags) == [0]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = vocabulary_cross_entropy(w, h, target)
+        ops.check_errors()
+        graph.replay()
+        assert torch.equal(held, want)
+        target[2] = 100                                               # outside the vocabulary: reported by the replay, once
+        graph.replay()
+        with pytest.raises(RuntimeError, match="index"):
+            ops.check_errors()
+        ops.check_errors()

@@ -25,6 +25,7 @@ def native(monkeypatch):
     lib = Native()
     monkeypatch.setattr(vocab, "load", lambda: lib)
     monkeypatch.setattr(vocab, "error_flag", lambda device: None)
+    monkeypatch.setattr(vocab, "_error_flags", {None: None})
     return lib
 
 
@@ -142,6 +143,7 @@ def test_tensors_without_memory_are_refused(entry, kind, monkeypatch):
     """Their address is null, or not to be had.  They are refused before the error word is made, which would be one of them."""
     from torch._subclasses.fake_tensor import FakeTensorMode
     monkeypatch.setattr(ops, "_error_flags", flags := {})
+    monkeypatch.setattr(vocab, "_error_flags", flags)
     with pytest.raises(ValueError, match="values in memory of its own"):
         if kind == "fake":
             with FakeTensorMode():
@@ -215,3 +217,15 @@ def test_scores_of_the_vocabulary_loss_are_fp32(ht, wt):
 def test_kernel_bench_sequences():
     from q38.utils.kernel_bench import sequences
     assert [sequences(t) for t in (1, 100, 4095, 4096, 10000, 16384)] == [(1, 1), (1, 100), (1, 4095), (1, 4096), (2, 4096), (4, 4096)]
+
+
+# ---- the error word --------------------------------------------------------------------------------------------------------------------------
+def test_the_error_word_is_not_made_in_a_capture(native, monkeypatch):
+    """Its zeros would be written by the replays: garbage before the first, and what a replay reported lost in the next."""
+    monkeypatch.setattr(vocab, "_error_flags", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        _call(torch.randn(5, 8))
+    monkeypatch.setattr(vocab, "_error_flags", {None: torch.zeros(1)})
+    _call(torch.randn(5, 8))
+    assert len(native.weights) == 1
