@@ -524,9 +524,13 @@ BwdShape bwd_shape(long long rows, int dim, bool packed16) {
 template <typename InT, typename OutT, int VEC>
 void launch_bwd(LnArgs& p, const BwdShape& s, cudaStream_t stream) {
   p.groups = s.groups;
-  const size_t smem = s.groups > 1 || p.dim > 8192 ? size_t(s.groups) * 2 * p.dim * 4 : 0;        // 96 KB at most
+  // Several groups: 64 KB at most.  One group with its sums in shared memory: both sums of the longest row.
+  constexpr int most = 2 * LN_LONGEST * 4;
+  static_assert(most <= 192 * 1024, "shared memory of a CTA, beside the scratch");
+  const size_t smem = s.groups > 1 || p.dim > 8192 ? size_t(s.groups) * 2 * p.dim * 4 : 0;
+  TORCH_CHECK(smem <= most, "layer_norm: shared memory of the backward");
   auto go = [&](auto kernel) {
-    if (smem > 40 * 1024) allow_shared_memory((const void*)kernel, 128 * 1024);
+    if (smem > 40 * 1024) allow_shared_memory((const void*)kernel, most);
     launch(kernel, (unsigned)s.ctas, s.G * s.groups, smem, stream, p);
   };
   if (p.dim <= 256) go(layer_norm_bwd_kernel<InT, OutT, VEC, 8, true, false>);

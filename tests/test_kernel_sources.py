@@ -128,3 +128,12 @@ def test_no_lane_skips_ahead_of_a_tensor_memory_read(name):
         condition = code[code.rfind("\n", 0, m.start()) + 1:m.start()] + " ".join(heads[loop + 1:])
         if re.search(r"tmem_(ld|st)_32", body) and not re.search(WARP_UNIFORM, condition):
             assert body.lstrip().startswith("__syncwarp();"), (name, condition)
+
+
+def test_layer_norm_allows_the_shared_memory_of_its_longest_row():
+    """Two fp32 sums per element of the longest row that a CTA holds; the allowance is derived from that length, not written beside it."""
+    code = code_of("layernorm.cu")
+    longest = int(re.search(r"constexpr int LN_LONGEST = (\d+);", code).group(1))
+    assert 2 * longest * 4 <= 227 * 1024 - 16 * 128 * 4                    # beside the backward's static scratch
+    most = re.search(r"allow_shared_memory\(\(const void\*\)kernel, (\w+)\)", code).group(1)
+    assert re.search(rf"constexpr int {most} = 2 \* LN_LONGEST \* 4;", code)
