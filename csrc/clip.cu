@@ -2,7 +2,8 @@
 //
 // Two launches for up to 512 tensors of any sizes: the tensors' addresses travel as kernel parameters (no table to copy to the device, so a captured
 // graph replays without host memory), and each CTA walks pieces of equal size of the whole list.
-//   norm    each CTA leaves its sum of squares in 64 bits: squares of fp32 values neither overflow nor vanish, and the order of additions is fixed
+//   norm    each CTA leaves its sum of squares in 64 bits, in a fixed order: squares of fp32 values are formed there too, so they neither overflow nor vanish; those of
+//           16-bit values, exact in fp32, are added by fours in fp32 first (clip_four)
 //   scale   each CTA adds up all sums in one order (a few KB from L2, instead of a third launch), takes the factor and scales its pieces
 // Bound by memory: one read for the norm, one read and one write for the scaling.  The scaling walks backwards, since what the norm read last is still in L2.
 // Where the factor is 1 and a tensor is its own result, there is nothing to write.

@@ -10,7 +10,7 @@
 // memory, CTAs by a second kernel in a fixed order (no atomics: the sums have the same bits in every run).  The next row is on its way while the current
 // one is reduced.  All sums are fp32.
 // Replayed on a B200: 16384 x 1024 bf16 forward 14.4 us (4.7 TB/s, 71 % of the copy bandwidth), backward with its sums 22.5 us (4.5 TB/s); 4096 x 2304 fp32 15.0 and
-// 22.9 us; 5001 x 2305 fp32, where rows are not on 16 bytes and elements come one by one, 18.9 and 29 us.
+// 22.9 us; 5001 x 2305 fp32, where rows are not on 16 bytes and elements come one by one, 18.9 and 29 us.  fp16 takes the times of bf16; 8192 x 1024 fp32 to bf16 12.0 and 17.7.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(ACC_SMEM ? 1024 : E == 32 ? 256 : E == 8 ? (VE
   }
 }
 
-// Rows of any length, a CTA each, read again for every sum (the row comes from L2).  The weight sums are kept in the CTA's part of `partial`.
+// Rows of any length, a CTA each, read again for every sum (the row comes from L2).  The weight sums are kept in the CTA's part of `partial`.  Bound by those reads, an
+// element per access: 1000 x 20000 bf16 forward 86 us, with backward 246 (floors 12 and 31).
 template <typename InT, typename OutT>
 __global__ void __launch_bounds__(1024) layer_norm_long_kernel(LnArgs p, bool backward) {
   grid_wait();

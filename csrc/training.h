@@ -33,7 +33,7 @@ at::Tensor vocab_rows(const at::Tensor& t);
 std::array<at::Tensor, 3> vocab_loss_fwd(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, at::IntArrayRef shape, int64_t reduction,
                                          const at::Tensor& err);
 // g: gradient of the loss ([rows] fp32 without a reduction, one element with one).  Returns {dh (bf16, or fp32 with `fp32_dh`), dW}: undefined where not wanted or, for dW,
-// where it was added to `grad` (fp32 [vocabulary, h], contiguous).  `workspace`: bytes that dz of one piece may take.
+// where it was added to `grad` (fp32 [vocabulary, h], contiguous).  `workspace`: bytes that dz of one piece may take; 256 columns are taken in any case.
 std::pair<at::Tensor, at::Tensor> vocab_loss_bwd(const at::Tensor& g, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, const at::Tensor& lse2,
                                                  const at::Tensor& count, int64_t reduction, bool want_dh, bool fp32_dh, bool want_dw, bool fp32_dw, const at::Tensor& grad, int64_t workspace,
                                                  const at::Tensor& err);

@@ -446,7 +446,7 @@ std::array<Tensor, 3> vocab_loss_fwd(const Tensor& hidden, const Tensor& weight,
   auto loss = new_tensor(reduction ? at::IntArrayRef(&rows, 1) : shape, at::kFloat, device), lse2 = new_tensor({rows}, at::kFloat, device);
   auto stream = at::cuda::getCurrentCUDAStream();
   if (rows) {
-    // 65536 rows at a time bound the pairs' workspace (a sixteenth of a byte per row and column)
+    // 65536 rows at a time bound the pairs' workspace: 16 bytes per row and tile of bn columns, so a sixteenth of a byte per score in wide tiles, a quarter in the narrowest
     for (int64_t at = 0; at < rows; at += 65536) {
       const int64_t n = std::min<int64_t>(65536, rows - at);
       const Tensor h = n == rows ? hidden : hidden.narrow(0, at, n);
@@ -489,7 +489,7 @@ std::pair<Tensor, Tensor> vocab_loss_bwd(const Tensor& g, const Tensor& h, const
     if (want_dw && !grad.defined()) dw = new_tensor({vocab, K}, dw_type, device).zero_();
     return {dh, dw};
   }
-  // Pieces: as few as the workspace allows, of equal width (whole tiles)
+  // Pieces: as few as the workspace allows, of equal width (whole tiles); 256 columns at least, which is more than 256 MB beyond 524288 rows
   const int64_t widest = std::max<int64_t>(256, workspace / (2 * rows) / 256 * 256), pieces = (vocab + widest - 1) / widest;
   const int64_t width = std::min((vocab + 7) / 8 * 8, ((vocab + pieces - 1) / pieces + 255) / 256 * 256);
   auto dz_all = new_tensor({rows, width}, at::kBFloat16, device);

@@ -34,12 +34,13 @@ def vocabulary_cross_entropy(weight, hidden, target, reduction="mean"):
     hidden: ``[..., h]`` bf16 or fp32 (rounded to bf16 for the products); weight: ``[vocabulary, h]`` bf16, or fp32 as a master weight (rounded to bf16 by every
     call, unless the trainer's arena keeps its bf16 form); target: int64 of
     hidden's leading shape, -100 where a row does not count (any other target outside the vocabulary counts as -100 and raises at
-    `q38.ops.check_errors`).  ``reduction``: ``"mean"`` over the rows that count (0 where none does), ``"sum"``, or ``"none"`` (fp32 losses of
+    `q38.ops.check_errors`; in host memory it raises at once).  ``reduction``: ``"mean"`` over the rows that count (0 where none does), ``"sum"``, or ``"none"`` (fp32 losses of
     target's shape, 0 where a row does not count).
 
     On a GPU the scores exist as one piece's bf16 gradients at most; scores, sums and losses are fp32, and results have the same bits in every
     run.  Where `linear_cross_entropy` keeps bf16 scores of all rows for the backward (vocabularies up to 16384), this forms them again: a third more
-    products for memory that does not grow with the vocabulary."""
+    products for memory that does not grow with the vocabulary.  First derivatives only, backward; capturable into a CUDA graph after a first call on the device;
+    fake and wrapped tensors are refused."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"vocabulary_cross_entropy: reduction must be mean, sum or none, got {reduction!r}")
     if hidden.is_cuda:

@@ -56,8 +56,8 @@ def rotary_frequencies(rotary_dim, theta=10000.0, scaling=None, device=None):
     * ``"linear"``: every angle divided by s (position interpolation);
     * ``"ntk"``: theta grows to ``theta * s ** (r / (r - 2))``, so the slowest pair turns s times slower and the fastest as before;
     * ``"yarn"``: pairs that make more than ``beta_fast`` turns (32) in ``original_max_position_embeddings`` positions stay, those below
-      ``beta_slow`` (1) are divided by s, with a ramp over the pairs between, whose ends are rounded outwards to whole pairs unless ``truncate`` is
-      false; the factor is ``attention_factor``, or ``0.1 ln s + 1`` (Peng et al., "YaRN", 2023)."""
+      ``beta_slow`` (1) are divided by s (Peng et al., "YaRN", 2023).  The ramp between is linear in the pair's index, as published models use it, where the paper's
+      is linear in the number of turns; its ends are rounded outwards to whole pairs unless ``truncate`` is false.  The factor is ``attention_factor``, or ``0.1 ln s + 1``."""
     _require(rotary_dim > 0 and rotary_dim % 2 == 0, "rotary_frequencies: an even number of rotated dimensions is required")
     _require(theta > 1, "rotary_frequencies: theta must be above 1")
     scaling = dict(scaling or {})
@@ -103,7 +103,8 @@ def rotary(q, k, positions, frequencies, magnitude=1.0, interleaved=False):
     q: ``[batch, seq, heads, dim]`` or ``[tokens, heads, dim]``; k: the same with a head count of its own, or None.  bf16, fp16 or fp32, any strides (a head-major
     tensor goes in as ``x.transpose(1, 2)``, a packed projection as slices); results have the layout of their input.  positions: whole numbers ``[seq]``
     or ``[batch, seq]`` (``[tokens]``), of any size and sign; angles are formed in 64 bits.  frequencies: ``rotary_dim / 2`` values in 64 bits
-    (`rotary_frequencies`), which get no gradient: ones that want it are refused; dimensions from rotary_dim on pass through.  A pair is ``(x[i], x[i + rotary_dim / 2])``, interleaved ``(x[2 i], x[2 i + 1])``."""
+    (`rotary_frequencies`), which get no gradient: ones that want it are refused.  Dimensions from rotary_dim on pass through.  A pair is
+    ``(x[i], x[i + rotary_dim / 2])``, interleaved ``(x[2 i], x[2 i + 1])``."""
     if q.dim() == 3:
         _require(k is None or k.dim() == 3, "rotary: queries and keys have the same number of dimensions")
         q2, k2 = rotary(q.unsqueeze(0), None if k is None else k.unsqueeze(0), positions, frequencies, magnitude, interleaved)
@@ -160,7 +161,7 @@ def _check_host(grads, out):
 def grad_norm(grads):
     """Global 2-norm of a list of fp32, bf16 and fp16 tensors (entries that are None are left out): a 0-dim fp32 tensor on their device.
 
-    Squares are added in 64 bits in a fixed order.  Tensors are dense in memory, in any layout and at any offset."""
+    Squares are added in 64 bits in a fixed order (on a GPU those of 16-bit values by fours in fp32 first, where they are exact).  Tensors are dense in memory, in any layout and at any offset."""
     grads, _ = _gradients(grads)
     if grads[0].is_cuda:
         return load().grad_norm(grads)

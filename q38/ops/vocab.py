@@ -3,7 +3,7 @@ import torch
 
 from . import _error_flags, error_flag, load
 
-# Bytes that the score gradients of one piece of the vocabulary may take.  A piece of 256 MB is written and read twice at the memory's rate while its three
+# Bytes that the score gradients of one piece of the vocabulary may take (a piece has 256 words at least: more than this beyond 524288 rows).  A piece of 256 MB is written and read twice at the memory's rate while its three
 # products take several times as long; smaller pieces only add launches and passes over the hidden gradient's sums.
 PIECE_BYTES = 256 << 20
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
